@@ -36,7 +36,7 @@ typedef struct rcu_kv rcu_kv;
 
 enum rcu_status {
     RCU_OK = 0,
-    RCU_ERR_INVALID = 1,     /* bad argument, shape or handle */
+    RCU_ERR_INVALID = 1,     /* bad argument, shape or handle; from rcu_check_device: bad device data (0x8) */
     RCU_ERR_CUDA = 2,        /* CUDA runtime error (message holds cudaGetErrorString) */
     RCU_ERR_UNSUPPORTED = 3, /* type/format not implemented on this path */
     RCU_ERR_OOM = 4,         /* device allocation failed */
@@ -187,6 +187,69 @@ RCU_API int32_t rcu_kv_import(rcu_ctx *ctx, rcu_kv *kv, const void *k_host, cons
 RCU_API int32_t rcu_attention(rcu_ctx *ctx, const rcu_kv *kv, const float *q_dev, uint64_t n_tok, uint64_t n_head,
                       uint64_t pos0, uint64_t window, float softcap, float *out_dev);
 
+/* ---- several sequences: paged KV cache and attention over a batch (no counterpart in the
+ * reference, whose caches hold one sequence each; the formula is that of rcu_attention) ----- */
+/* A pool of n_pages pages shared by any number of sequences. A page holds page_size positions
+ * (a power of two, 16..1024) of one sequence for every KV head: [page][kv head][slot][head_dim]
+ * f16 (kv_type RCU_KV_F16; the other formats return RCU_ERR_UNSUPPORTED), head_dim a multiple of
+ * 32 up to 256. k_dev / v_dev: the caller's pools of n_pages * n_head_kv * page_size * head_dim
+ * f16 each (16-byte aligned, not copied, not freed), or both NULL: the library allocates zeroed
+ * ones. Which page belongs to whom is the caller's bookkeeping. */
+typedef struct rcu_paged rcu_paged;
+RCU_API int32_t rcu_paged_create(rcu_ctx *ctx, int32_t kv_type, uint64_t n_head_kv, uint64_t head_dim,
+                                 uint64_t page_size, uint64_t n_pages, void *k_dev, void *v_dev, rcu_paged **out);
+RCU_API void rcu_paged_free(rcu_paged *pg);
+RCU_API int32_t rcu_paged_device_ptrs(const rcu_paged *pg, void **k_dev, void **v_dev);
+/* One batch of new tokens of n_seq sequences. The arrays are device memory that is read when the
+ * kernels run, so a captured graph replays with what they hold then; n_tok, n_seq and ld_pages
+ * are fixed by the capture. What the kernels find out of range there (offsets that fall or leave
+ * the batch, a len below the sequence's new tokens or above its table, a page number outside the
+ * pool) they skip, read as zeros or clamp, never follow; rcu_sync / rcu_check_device then return
+ * RCU_ERR_INVALID (error bit 0x8). */
+typedef struct rcu_seqs {
+    const int32_t *cu;    /* [n_seq + 1]: rows cu[i] .. cu[i + 1] - 1 are sequence i's new tokens (none: equal) */
+    const int32_t *len;   /* [n_seq]: positions of sequence i, its new tokens the last of them */
+    const int32_t *pages; /* [n_seq][ld_pages]: position P of sequence i is in page pages[i][P / page_size] */
+    uint64_t n_seq, n_tok, ld_pages;
+    uint64_t max_len;     /* the longest len, 0 when unknown: shapes the launch, never the results */
+} rcu_seqs;
+/* Appends the new tokens' keys and values (post-RoPE keys; rows of n_head_kv * head_dim values of
+ * ggml type F32, F16 or BF16, ld values apart, every row on a 16-byte boundary), rounded once to
+ * f16. Rows behind the last sequence are ignored. */
+RCU_API int32_t rcu_paged_store(rcu_ctx *ctx, rcu_paged *pg, const rcu_seqs *seqs, const void *k_dev,
+                                const void *v_dev, uint32_t type, uint64_t ld);
+/* Causal grouped-query attention of the new tokens over their sequences' pages, the new tokens'
+ * own keys and values (already stored) among them: any mix of single tokens and chunks in one
+ * call. q_dev: n_tok rows of n_head * head_dim values (F32 or F16, already scaled by attn_scale),
+ * ld_q apart; out_dev the same type, ld_out apart. window and softcap as in rcu_attention. Out rows
+ * behind the last sequence stay as they were. Masked keys and values do not count, whatever they
+ * hold. No workspace: calls may overlap on any streams. */
+RCU_API int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *seqs, const void *q_dev,
+                                    uint32_t type, uint64_t ld_q, uint64_t n_head, uint64_t window, float softcap,
+                                    void *out_dev, uint64_t ld_out);
+/* Causal grouped-query attention of whole prompts that lie one behind the other, without a cache:
+ * rows cu[i] .. cu[i + 1] - 1 (device, n_seq + 1 offsets) attend among themselves. q (F32 or F16
+ * over F16 keys and values, or BF16 over BF16; already scaled), k, v and out are rows ld_q / ld_kv /
+ * ld_out values apart, so slices of a fused projection do. max_len: the longest prompt, 0 when
+ * unknown (shapes the launch only). */
+RCU_API int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, uint64_t ld_q,
+                                     const void *k_dev, const void *v_dev, uint32_t kv_elem, uint64_t ld_kv,
+                                     const int32_t *cu, uint64_t n_seq, uint64_t n_tok, uint64_t max_len,
+                                     uint64_t n_head, uint64_t n_head_kv, uint64_t head_dim, uint64_t window,
+                                     float softcap, void *out_dev, uint64_t ld_out);
+
+/* ---- scores (no counterpart in the reference: its samplers take the logits on the host) ------ */
+/* For each of n_rows rows of n_vocab logits (F32, F16 or BF16, ld values apart):
+ *   logprob[r]  = log softmax(row)[targets[r]], 0 for target -1 (none); any other target outside
+ *                 the vocabulary gives NaN and error bit 0x8 (targets and logprob may both be NULL)
+ *   entropy[r]  = entropy of softmax(row) in nats (may be NULL)
+ *   top_ids[r][0 .. top_k-1], top_logprobs[r][..]: the top_k (0..128) largest, ties to the lowest index
+ * A row that holds NaN or +inf, or nothing above -inf, has no distribution: its log probabilities
+ * and entropy are NaN; top_ids still order its values, NaN as the largest. */
+RCU_API int32_t rcu_logprobs(rcu_ctx *ctx, const void *logits_dev, uint32_t type, uint64_t n_rows, uint64_t n_vocab,
+                             uint64_t ld, const int32_t *targets_dev, float *logprob_dev, float *entropy_dev,
+                             uint64_t top_k, int32_t *top_ids_dev, float *top_logprobs_dev);
+
 /* ---- transformer forward (model/mod.rs Model + Backend trait, model/cpu.rs) --------- */
 typedef struct rcu_model rcu_model;
 typedef struct rcu_backend rcu_backend;
@@ -232,6 +295,13 @@ RCU_API int32_t rcu_backend_forward(rcu_backend *b, const uint32_t *tokens, uint
 /* Same on device buffers, asynchronous on the context stream (tokens_dev: n uint32). */
 RCU_API int32_t rcu_backend_forward_device(rcu_backend *b, const uint32_t *tokens_dev, uint64_t n, uint64_t pos,
                                            int32_t all_logits, float *logits_dev);
+/* rcu_backend_forward of n tokens, scored on the device: instead of every row's logits the host
+ * gets what rcu_logprobs makes of them (targets: n token ids or -1, may be NULL with logprob;
+ * entropy may be NULL; top_ids and top_logprobs hold n * top_k). Host buffers; synchronous. Appends
+ * to the KV cache as rcu_backend_forward does. */
+RCU_API int32_t rcu_backend_score(rcu_backend *b, const uint32_t *tokens, uint64_t n, uint64_t pos,
+                                  const int32_t *targets, float *logprob, float *entropy, uint64_t top_k,
+                                  int32_t *top_ids, float *top_logprobs);
 /* Partial forward (no counterpart in the reference): layers [layer0, layer1) for n tokens at
  * positions pos..pos+n-1, starting from hidden rows x_dev (n x n_embd f32, device) instead of
  * the token embeddings; those layers' KV caches are appended as by rcu_backend_forward. Writes

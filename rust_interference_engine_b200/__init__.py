@@ -13,6 +13,9 @@ argument meaning:
   turbo::{row_bytes_4, quantize_4, Rotation}     turbo.row_bytes_4 / quantize_4 / rotate
   model::cpu::{KvType, LayerCache, attention}    KvType / LayerCache / attention
 
+Several sequences at once, which the reference's caches and samplers do not hold: PagedCache and
+SeqBatch with paged_attention, packed_attention over whole prompts, and logprobs.
+
 Device memory is passed as torch CUDA tensors (or raw device pointers); torch is only the
 allocator and stream plumbing. There is no CPU fallback: without the CUDA library or a
 GPU every call raises.
@@ -25,11 +28,11 @@ from dataclasses import dataclass
 from typing import Iterable, Sequence
 
 from . import _lib
-from ._lib import RcuError, RcuJob
+from ._lib import RcuError, RcuJob, RcuSeqs
 
 __all__ = ["GgmlType", "ActFormat", "KvType", "Rounding", "PrefillGemm", "Context", "Weight", "QuantActs", "MatmulJob",
            "matmul", "matmul_multi", "matmul_f32_static", "formats_for", "block_sums", "quantize_weight", "LayerCache",
-           "attention", "turbo", "RcuError"]
+           "attention", "PagedCache", "SeqBatch", "paged_attention", "packed_attention", "logprobs", "turbo", "RcuError"]
 
 
 class GgmlType(enum.IntEnum):  # quant/mod.rs:15-68 (GGUF ids)
@@ -150,7 +153,7 @@ class Context:
     def device_error_bits(self) -> int:
         bits = C.c_uint32(0)
         st = self._lib.rcu_check_device(self.ptr, C.byref(bits))
-        if st not in (0, _lib.RCU_ERR_TIMEOUT):
+        if st != 0 and not bits.value:
             _check(self.ptr, st)
         return int(bits.value)
 
@@ -377,6 +380,171 @@ def attention(ctx: Context, cache: LayerCache, q, n_tok: int, n_head: int, pos0:
     """Causal GQA attention over the cache (model/cpu.rs:552-634); q already x attn_scale."""
     _check(ctx.ptr, ctx._lib.rcu_attention(ctx.ptr, cache.ptr, C.c_void_p(_dptr(q)), n_tok, n_head, pos0, window,
                                            float(softcap or 0.0), C.c_void_p(_dptr(out))))
+
+
+def _elem(x) -> GgmlType:
+    """GGUF type id of a tensor's elements."""
+    ty = {"torch.float32": GgmlType.F32, "torch.float16": GgmlType.F16, "torch.bfloat16": GgmlType.BF16}.get(str(x.dtype))
+    if ty is None:
+        raise ValueError(f"f32, f16 or bf16 values expected, not {x.dtype}")
+    return ty
+
+
+def _on(ctx: Context, x, what: str) -> int:
+    """Device address of a tensor that must live on the context's device."""
+    if not x.is_cuda:
+        raise ValueError(f"{what}: expected a CUDA tensor")
+    if x.get_device() != ctx.device:
+        raise ValueError(f"{what}: on device {x.get_device()}, the context is on {ctx.device}")
+    return x.data_ptr()
+
+
+def _rows(ctx: Context, x, n: int, width: int, what: str):
+    """(address, type, row stride) of n rows of `width` values; the rows may be slices of wider
+    ones, their values must be contiguous."""
+    if x.dim() != 2 or x.shape[0] != n or x.shape[1] != width:
+        raise ValueError(f"{what}: expected {n} x {width} values, not {tuple(x.shape)}")
+    if x.stride(1) != 1 and width > 1:
+        raise ValueError(f"{what}: the values of a row must be contiguous")
+    return _on(ctx, x, what), _elem(x), x.stride(0) if n > 1 else max(x.stride(0), width)
+
+
+def _vector(ctx: Context, x, dtype: str, shape, what: str) -> int:
+    if str(x.dtype) != dtype or tuple(x.shape) != tuple(shape) or not x.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, not {x.dtype} {tuple(x.shape)}")
+    return _on(ctx, x, what)
+
+
+class SeqBatch:
+    """The new tokens of several sequences (rcu_seqs): rows cu[i] .. cu[i + 1] - 1 of a batch of
+    n_tok rows are sequence i's, len[i] counts its positions with them, pages[i] lists its pages.
+
+    cu (n_seq + 1), len (n_seq) and pages (n_seq x width) are int32 CUDA tensors; the kernels read
+    them when they run, so a captured graph replays with what they hold then. max_len (the longest
+    len, when the program knows it) shapes the launches, never the results."""
+
+    def __init__(self, cu, len, pages, n_tok: int, max_len: int = 0):  # noqa: A002
+        for x, what, dims in ((cu, "cu", 1), (len, "len", 1), (pages, "pages", 2)):
+            if str(x.dtype) != "torch.int32" or x.dim() != dims or not x.is_contiguous():
+                raise ValueError(f"{what}: expected a contiguous {dims}-dimensional int32 tensor")
+            if not x.is_cuda or x.get_device() != cu.get_device():
+                raise ValueError(f"{what}: expected a CUDA tensor on the batch's device")
+        n_seq = len.shape[0]
+        if cu.shape[0] != n_seq + 1 or pages.shape[0] != n_seq:
+            raise ValueError(f"{n_seq} sequences need {n_seq + 1} offsets and {n_seq} rows of pages")
+        if n_tok < 0 or max_len < 0:
+            raise ValueError("n_tok and max_len must not be negative")
+        self.n_seq, self.n_tok, self.device = n_seq, n_tok, cu.get_device()
+        self._keep = (cu, len, pages)
+        self._c = RcuSeqs(cu.data_ptr(), len.data_ptr(), pages.data_ptr(), n_seq, n_tok, pages.shape[1], max_len)
+        self._ref = C.byref(self._c)
+
+    def _on(self, ctx: Context):
+        if self.device != ctx.device:
+            raise ValueError(f"batch: on device {self.device}, the context is on {ctx.device}")
+        return self._ref
+
+
+class PagedCache:
+    """A pool of key / value pages for any number of sequences, [page][kv_head][slot][head_dim] f16
+    (rcu_paged_create). k and v: the program's own pools (f16 CUDA tensors of that many values),
+    or the library's when left out."""
+
+    def __init__(self, ctx: Context, n_head_kv: int, head_dim: int, page_size: int, n_pages: int,
+                 ty: KvType = KvType.F16, k=None, v=None):
+        self.ctx, self.ty, self.n_head_kv, self.head_dim = ctx, KvType(ty), n_head_kv, head_dim
+        self.page_size, self.n_pages = page_size, n_pages
+        self.ptr = C.c_void_p()
+        if (k is None) != (v is None):
+            raise ValueError("pass both pools or neither")
+        for x, what in ((k, "k"), (v, "v")):
+            if x is None:
+                continue
+            if _elem(x) != GgmlType.F16 or not x.is_contiguous() or x.numel() != n_pages * n_head_kv * page_size * head_dim:
+                raise ValueError(f"{what}: expected {n_pages * n_head_kv * page_size * head_dim} contiguous f16 values")
+            _on(ctx, x, what)
+        self._keep = (k, v)
+        _check(ctx.ptr, ctx._lib.rcu_paged_create(ctx.ptr, int(ty), n_head_kv, head_dim, page_size, n_pages,
+                                                  k.data_ptr() if k is not None else None,
+                                                  v.data_ptr() if v is not None else None, C.byref(self.ptr)))
+
+    def store(self, batch: SeqBatch, k, v) -> None:
+        """Append the batch's keys and values (n_tok x n_head_kv*head_dim f32, f16 or bf16)."""
+        ctx, width = self.ctx, self.n_head_kv * self.head_dim
+        kp, ty, ld = _rows(ctx, k, batch.n_tok, width, "k")
+        vp, ty_v, ld_v = _rows(ctx, v, batch.n_tok, width, "v")
+        if ty != ty_v or ld != ld_v:
+            raise ValueError("k and v must have the same type and row stride")
+        _check(ctx.ptr, ctx._lib.rcu_paged_store(ctx.ptr, self.ptr, batch._on(ctx), kp, vp, ty, ld))
+
+    def data_ptrs(self):
+        k, v = C.c_void_p(), C.c_void_p()
+        _check(self.ctx.ptr, self.ctx._lib.rcu_paged_device_ptrs(self.ptr, C.byref(k), C.byref(v)))
+        return int(k.value), int(v.value)
+
+    def free(self) -> None:
+        if getattr(self, "ptr", None):
+            self.ctx._lib.rcu_paged_free(self.ptr)
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def paged_attention(ctx: Context, cache: PagedCache, batch: SeqBatch, q, n_head: int, out, window: int = 0,
+                    softcap: float | None = None) -> None:
+    """Causal GQA attention of the batch's new tokens over their pages (rcu_paged_attention); q
+    (n_tok x n_head*head_dim, f32 or f16) already x attn_scale, out the same type."""
+    width = n_head * cache.head_dim
+    qp, ty, ld = _rows(ctx, q, batch.n_tok, width, "q")
+    op, ty_o, ld_o = _rows(ctx, out, batch.n_tok, width, "out")
+    if ty_o != ty:
+        raise ValueError("q and out must have the same type")
+    _check(ctx.ptr, ctx._lib.rcu_paged_attention(ctx.ptr, cache.ptr, batch._on(ctx), qp, ty, ld, n_head, window,
+                                                 softcap or 0.0, op, ld_o))
+
+
+def packed_attention(ctx: Context, q, k, v, cu, n_head: int, n_head_kv: int, head_dim: int, out, window: int = 0,
+                     softcap: float | None = None, max_len: int = 0) -> None:
+    """Causal GQA attention within each of the packed prompts, rows cu[i] .. cu[i + 1] - 1
+    (rcu_packed_attention): q (already x attn_scale) and out f32 or f16 over f16 k and v, or all bf16."""
+    n_tok = q.shape[0]
+    qp, ty, ld = _rows(ctx, q, n_tok, n_head * head_dim, "q")
+    kp, ty_k, ld_k = _rows(ctx, k, n_tok, n_head_kv * head_dim, "k")
+    vp, ty_v, ld_v = _rows(ctx, v, n_tok, n_head_kv * head_dim, "v")
+    op, ty_o, ld_o = _rows(ctx, out, n_tok, n_head * head_dim, "out")
+    if ty_k != ty_v or ld_k != ld_v or ty_o != ty:
+        raise ValueError("k and v must have the same type and row stride, q and out the same type")
+    n_seq = cu.shape[0] - 1
+    _check(ctx.ptr, ctx._lib.rcu_packed_attention(ctx.ptr, qp, ty, ld, kp, vp, ty_k, ld_k,
+                                                  _vector(ctx, cu, "torch.int32", (n_seq + 1,), "cu"), n_seq, n_tok,
+                                                  max_len, n_head, n_head_kv, head_dim, window, softcap or 0.0, op, ld_o))
+
+
+def logprobs(ctx: Context, logits, targets=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None) -> None:
+    """Scores of rows of logits (n_rows x n_vocab, f32, f16 or bf16) into the tensors that are given
+    (rcu_logprobs): logprob of targets (int32, -1: none), entropy (both n_rows f32), and the
+    largest top_k as top_ids (n_rows x top_k int32) and top_logprobs (n_rows x top_k f32)."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits: expected rows, not {tuple(logits.shape)}")
+    n, width = logits.shape
+    lp, ty, ld = _rows(ctx, logits, n, width, "logits")
+    if (targets is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
+        raise ValueError("pass targets with logprob, and top_ids with top_logprobs")
+    top_k = 0 if top_ids is None else top_ids.shape[-1]
+
+    def arg(x, dtype, shape, what):
+        return None if x is None else _vector(ctx, x, dtype, shape, what)
+
+    ids = arg(top_ids, "torch.int32", (n, top_k), "top_ids")
+    tlp = arg(top_logprobs, "torch.float32", (n, top_k), "top_logprobs")
+    _check(ctx.ptr, ctx._lib.rcu_logprobs(ctx.ptr, lp, ty, n, width, ld, arg(targets, "torch.int32", (n,), "targets"),
+                                          arg(logprob, "torch.float32", (n,), "logprob"),
+                                          arg(entropy, "torch.float32", (n,), "entropy"), top_k, ids if top_k else None,
+                                          tlp if top_k else None))
 
 
 class turbo:  # noqa: N801  (namespace mirroring turbo.rs)

@@ -52,6 +52,14 @@ SIGNATURES = {
     "rcu_kv_export": (I32, [P, P, P, P]),
     "rcu_kv_import": (I32, [P, P, P, P]),
     "rcu_attention": (I32, [P, P, P, U64, U64, U64, U64, F, P]),
+    "rcu_paged_create": (I32, [P, I32, U64, U64, U64, U64, P, P, C.POINTER(P)]),
+    "rcu_paged_free": (None, [P]),
+    "rcu_paged_device_ptrs": (I32, [P, C.POINTER(P), C.POINTER(P)]),
+    "rcu_paged_store": (I32, [P, P, P, P, P, U32, U64]),
+    "rcu_paged_attention": (I32, [P, P, P, P, U32, U64, U64, U64, F, P, U64]),
+    "rcu_packed_attention": (I32, [P, P, U32, U64, P, P, U32, U64, P, U64, U64, U64, U64, U64, U64, U64, F, P, U64]),
+    "rcu_logprobs": (I32, [P, P, U32, U64, U64, U64, P, P, P, U64, P, P]),
+    "rcu_backend_score": (I32, [P, P, U64, U64, P, P, P, U64, P, P]),
     "rcu_model_create": (I32, [P, P, C.POINTER(P)]),
     "rcu_model_free": (None, [P]),
     "rcu_model_set_tensor": (I32, [P, C.c_char_p, U32, U64, U64, P]),
@@ -76,6 +84,11 @@ SIGNATURES = {
 
 class RcuJob(C.Structure):
     _fields_ = [("w", C.c_void_p), ("out", C.c_void_p), ("ld", C.c_uint64)]
+
+
+class RcuSeqs(C.Structure):
+    _fields_ = [("cu", C.c_void_p), ("len", C.c_void_p), ("pages", C.c_void_p), ("n_seq", C.c_uint64),
+                ("n_tok", C.c_uint64), ("ld_pages", C.c_uint64), ("max_len", C.c_uint64)]
 
 
 class RcuError(RuntimeError):

@@ -35,16 +35,6 @@ static uint64_t row_bytes(int t, uint64_t cols) {
 
 using namespace rcu;
 
-#define RCU_GUARD_BEGIN try {
-#define RCU_GUARD_END(ctx)                                              \
-    }                                                                   \
-    catch (const std::bad_alloc &) {                                    \
-        return set_err((ctx), RCU_ERR_OOM, "host allocation failed");   \
-    }                                                                   \
-    catch (...) {                                                       \
-        return set_err((ctx), RCU_ERR_RUNTIME, "internal exception");   \
-    }
-
 namespace rcu {
 cudaError_t prefer_max_shared(const void *kern) {
     // kernels already configured on the current device; a handful of entries
@@ -158,6 +148,10 @@ int32_t rcu_check_device(rcu_ctx *ctx, uint32_t *bits_out) {
     if (bits) {
         RCU_CUDA_TRY(ctx, cudaMemsetAsync(ctx->dev_err, 0, sizeof(uint32_t), ctx->stream));
         char m[96];
+        if (bits == ERR_BAD_ARG) {
+            std::snprintf(m, sizeof m, "device data out of range (error bits 0x%x)", bits);
+            return set_err(ctx, RCU_ERR_INVALID, m);
+        }
         std::snprintf(m, sizeof m, "bounded device wait expired (error bits 0x%x)", bits);
         return set_err(ctx, RCU_ERR_TIMEOUT, m);
     }

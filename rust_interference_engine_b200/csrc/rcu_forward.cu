@@ -69,6 +69,8 @@ struct rcu_backend {
     // that both copies run as DMA instead of through the driver's pageable staging
     uint32_t *tok_pin = nullptr;
     float *logits_pin = nullptr;
+    uint32_t *score_dev = nullptr, *score_pin = nullptr;  // rcu_backend_score's results
+    uint64_t score_words = 0;
     uint32_t ep_e0 = 0, ep_n = 0xffffffffu;  // experts of this rank: [ep_e0, ep_e0 + ep_n)
     rcu_acts *acts2 = nullptr;
     bool ar_ok = false;
@@ -1673,6 +1675,8 @@ void rcu_backend_free(rcu_backend *b) {
     if (b->moe_off_host) cudaFreeHost(b->moe_off_host);
     if (b->tok_pin) cudaFreeHost(b->tok_pin);
     if (b->logits_pin) cudaFreeHost(b->logits_pin);
+    if (b->score_dev) cudaFree(b->score_dev);
+    if (b->score_pin) cudaFreeHost(b->score_pin);
     if (b->stream) cudaStreamDestroy(b->stream);
     for (auto *kv : b->kv) rcu_kv_free(kv);
     rcu_acts_free(b->acts);
@@ -1792,6 +1796,67 @@ int32_t rcu_backend_forward_device(rcu_backend *b, const uint32_t *tokens_dev, u
         RCU_CUDA_TRY(b->ctx, cudaMemcpyAsync(logits_dev, b->logits, b->m->cfg.n_vocab * 4, cudaMemcpyDeviceToDevice,
                                              b->ctx->stream));
     return RCU_OK;
+}
+
+int32_t rcu_backend_score(rcu_backend *b, const uint32_t *tokens, uint64_t n, uint64_t pos, const int32_t *targets,
+                          float *logprob, float *entropy, uint64_t top_k, int32_t *top_ids, float *top_logprobs) {
+    if (!b || !tokens) return b ? set_err(b->ctx, RCU_ERR_INVALID, "null argument") : RCU_ERR_INVALID;
+    if (!targets != !logprob) return set_err(b->ctx, RCU_ERR_INVALID, "score: pass targets and logprob, or neither");
+    if (top_k && (!top_ids || !top_logprobs)) return set_err(b->ctx, RCU_ERR_INVALID, "score: top_k without its outputs");
+    const uint64_t nv = b->m->cfg.n_vocab;
+    if (top_k > 128 || top_k > nv)
+        return set_err(b->ctx, RCU_ERR_INVALID, "score: at most 128 alternatives, and no more than the vocabulary");
+    if (int32_t st = check_forward(b, n, pos)) return st;
+    for (uint64_t i = 0; i < n; i++) {
+        if (tokens[i] >= b->embd->rows) return set_err(b->ctx, RCU_ERR_RUNTIME, "token id " + std::to_string(tokens[i]) + " out of range");
+        if (targets && (targets[i] < -1 || targets[i] >= (int64_t)nv))
+            return set_err(b->ctx, RCU_ERR_RUNTIME, "target id " + std::to_string(targets[i]) + " out of range");
+    }
+    RCU_GUARD_BEGIN
+    rcu_ctx *ctx = b->ctx;
+    DeviceGuard guard(ctx);
+    // results of one call, device and pinned host side by side: targets, logprob, entropy (max_batch
+    // words each), then the alternatives; made by the first call that needs them and grown by top_k
+    const uint64_t words = b->max_batch * (3 + 2 * top_k);
+    if (words > b->score_words) {
+        if (b->score_dev) cudaFree(b->score_dev);
+        if (b->score_pin) cudaFreeHost(b->score_pin);
+        b->score_dev = b->score_pin = nullptr;
+        b->score_words = 0;
+        RCU_CUDA_TRY(ctx, cudaMalloc(&b->score_dev, words * 4));
+        RCU_CUDA_TRY(ctx, cudaMallocHost(&b->score_pin, words * 4));
+        b->score_words = words;
+    }
+    if (!b->tok_pin) RCU_CUDA_TRY(ctx, cudaMallocHost(&b->tok_pin, b->max_batch * sizeof(uint32_t)));
+    std::memcpy(b->tok_pin, tokens, n * sizeof(uint32_t));  // the previous call synchronised: staging is free
+    uint32_t *dev = b->score_dev, *pin = b->score_pin;
+    const uint64_t T = n;  // targets | logprob | entropy | ids | top logprobs, n rows each
+    if (targets) std::memcpy(pin, targets, T * 4);
+    int32_t st = run_forward(b, b->tok_pin, true, n, pos, n > 1, b->logits);
+    cudaError_t e = cudaSuccess;
+    if (st == RCU_OK) {
+        if (targets) e = cudaMemcpyAsync(dev, pin, T * 4, cudaMemcpyHostToDevice, ctx->stream);
+        const LogprobParams lp{b->logits, targets ? (const int32_t *)dev : nullptr, logprob ? (float *)(dev + T) : nullptr,
+                               entropy ? (float *)(dev + 2 * T) : nullptr, (float *)(dev + 3 * T + T * top_k),
+                               (int32_t *)(dev + 3 * T), nv, (uint32_t)n, (uint32_t)nv, (uint32_t)top_k, ctx->dev_err};
+        if (e == cudaSuccess) st = launch_logprobs(ctx, lp, T_F32);
+        if (st == RCU_OK && e == cudaSuccess)
+            e = cudaMemcpyAsync(pin, dev, T * (3 + 2 * top_k) * 4, cudaMemcpyDeviceToHost, ctx->stream);
+    }
+    if (st || e != cudaSuccess) {
+        cudaStreamSynchronize(b->stream);  // copies from the staging buffers must finish before their next use
+        cudaStreamSynchronize(ctx->stream);
+        return st ? st : cuda_err(ctx, e, "score copies");
+    }
+    if ((st = rcu_sync(ctx))) return st;
+    if (logprob) std::memcpy(logprob, pin + T, T * 4);
+    if (entropy) std::memcpy(entropy, pin + 2 * T, T * 4);
+    if (top_k) {
+        std::memcpy(top_ids, pin + 3 * T, T * top_k * 4);
+        std::memcpy(top_logprobs, pin + 3 * T + T * top_k, T * top_k * 4);
+    }
+    return RCU_OK;
+    RCU_GUARD_END(b->ctx)
 }
 
 int32_t rcu_backend_forward_layers(rcu_backend *b, const float *x_dev, uint64_t n, uint64_t pos, uint64_t layer0,

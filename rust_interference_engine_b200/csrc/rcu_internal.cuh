@@ -285,3 +285,14 @@ inline cudaError_t launch_k(const rcu_ctx *ctx, void (*kern)(KArgs...), dim3 gri
         cudaError_t _e = (expr);                                          \
         if (_e != cudaSuccess) return rcu::cuda_err((ctx), _e, #expr);    \
     } while (0)
+
+// Nothing throws across the C ABI.
+#define RCU_GUARD_BEGIN try {
+#define RCU_GUARD_END(ctx)                                              \
+    }                                                                   \
+    catch (const std::bad_alloc &) {                                    \
+        return rcu::set_err((ctx), RCU_ERR_OOM, "host allocation failed");   \
+    }                                                                   \
+    catch (...) {                                                       \
+        return rcu::set_err((ctx), RCU_ERR_RUNTIME, "internal exception");   \
+    }

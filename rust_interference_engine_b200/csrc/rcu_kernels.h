@@ -116,4 +116,42 @@ uint64_t attention_scratch_bytes(const rcu_kv *kv, uint64_t n_tok, uint64_t n_he
 uint64_t attention_scratch_bytes_upto(const rcu_ctx *ctx, const rcu_kv *kv, uint64_t max_batch, uint64_t n_head,
                                       uint64_t window);
 
+
+// Attention over a batch of sequences (rcu_attn_seq.cu). kv: the tensors that the tiled loads
+// read, rows of hd elements: the page pool's rows [page][kv head][slot], or packed prompt rows with
+// a stride between kv heads. max_len shapes the launch only.
+struct SeqAttnParams;
+struct SeqKvDesc {
+    const void *k, *v;
+    bool pages;
+    uint64_t rows, row_stride, head_stride;  // strides in elements
+};
+int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, int kv_type, const SeqKvDesc &kv,
+                         uint64_t max_len);
+// log p of targets, entropy and the largest top_k of rows of logits (rcu_logprobs.cu).
+struct LogprobParams {
+    const void *logits;
+    const int32_t *targets;
+    float *logprob, *entropy, *top_logprobs;
+    int32_t *top_ids;
+    uint64_t ld;
+    uint32_t rows, vocab, top_k;
+    uint32_t *err;
+};
+int launch_logprobs(rcu_ctx *ctx, const LogprobParams &p, int type);
+
+// Makes the context's device the current one for the length of a call.
+struct DeviceGuard {
+    int prev = -1, dev;
+    explicit DeviceGuard(const rcu_ctx *ctx) : dev(ctx->device) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) cudaSetDevice(dev);
+    }
+    ~DeviceGuard() {
+        if (prev >= 0 && prev != dev) cudaSetDevice(prev);
+    }
+    DeviceGuard(const DeviceGuard &) = delete;
+    DeviceGuard &operator=(const DeviceGuard &) = delete;
+};
+
 }  // namespace rcu

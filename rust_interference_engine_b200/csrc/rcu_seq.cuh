@@ -1,0 +1,229 @@
+// rcu_seq.cuh -- what the kernels over a batch of sequences share: the batch's description, the
+// lookup of a work tile's sequence, element conversion, and the row-by-row attention that the
+// tiled kernels fall back to for rows with values that are not finite.
+//
+// A batch is `n_tok` rows of new tokens; rows cu[i] .. cu[i + 1] - 1 belong to sequence i, whose
+// last new token has position len[i] - 1. All of it is device memory that the host never reads, so
+// every kernel clamps what it takes from there before it forms an address: a wrong value costs an
+// error bit (ERR_BAD_ARG) and rows without a meaning, never an access out of range.
+#pragma once
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "rcu_internal.cuh"
+
+namespace rcu {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct SeqView {
+    const int32_t *cu;     // [n_seq + 1]
+    const int32_t *len;    // [n_seq]; nullptr: a sequence is its new tokens (packed prompts)
+    const int32_t *pages;  // [n_seq][ld_pages]; nullptr: keys and values are packed rows
+    uint32_t n_seq, n_tok, ld_pages, n_pages, page_shift;
+    uint32_t *err;
+};
+
+// What one sequence of the batch is, clamped to the batch and to its page table.
+struct SeqSpan {
+    uint32_t seq, first, n_new;  // rows first .. first + n_new - 1
+    int64_t len;                 // positions 0 .. len - 1 are in the cache
+    // position of new token t: negative where a wrong len is shorter than n_new (no keys then)
+    __device__ __forceinline__ int64_t pos(uint32_t t) const { return len - (int64_t)n_new + (int64_t)t; }
+};
+
+__device__ __forceinline__ uint32_t seq_rows(const SeqView &b, uint32_t s, uint32_t *first) {
+    const int32_t c0 = b.cu[s], c1 = b.cu[s + 1];
+    const int32_t a0 = min(max(c0, 0), (int32_t)b.n_tok), a1 = min(max(c1, a0), (int32_t)b.n_tok);
+    if (a0 != c0 || a1 != c1) atomicOr(b.err, (uint32_t)ERR_BAD_ARG);
+    *first = (uint32_t)a0;
+    return (uint32_t)(a1 - a0);
+}
+__device__ __forceinline__ int64_t seq_len(const SeqView &b, uint32_t s, uint32_t n_new) {
+    if (!b.len) return n_new;
+    const int64_t cap = (int64_t)b.ld_pages << b.page_shift, l = b.len[s];
+    if (l < (int64_t)n_new || l > cap) atomicOr(b.err, (uint32_t)ERR_BAD_ARG);
+    return min(max(l, (int64_t)0), cap);
+}
+
+// The sequence that holds work tile `ti` when sequence i takes ceil(n_new[i] * group / rows) tiles,
+// and the tile's number within it; false behind the last tile. One whole warp; the scan reads
+// 2 * n_seq words that stay in L1 / L2.
+__device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, uint32_t rows, uint32_t ti, SeqSpan *sp,
+                                              uint32_t *tile) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t base = 0;
+    for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 32) {
+        uint32_t first = 0, n = 0;
+        if (s0 + lane < b.n_seq) n = seq_rows(b, s0 + lane, &first);
+        const uint32_t t = (uint32_t)(((uint64_t)n * group + rows - 1) / rows);
+        uint32_t inc = t;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= (uint32_t)d) inc += v;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, ti - base < inc);  // ti >= base here
+        if (hit) {
+            const int l = __ffs((int)hit) - 1;
+            sp->seq = s0 + l;
+            sp->first = __shfl_sync(0xffffffffu, first, l);
+            sp->n_new = __shfl_sync(0xffffffffu, n, l);
+            *tile = ti - base - (__shfl_sync(0xffffffffu, inc, l) - __shfl_sync(0xffffffffu, t, l));
+            sp->len = seq_len(b, sp->seq, sp->n_new);
+            return true;
+        }
+        base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return false;
+}
+// An upper bound of the tiles of a batch, from what the host knows.
+inline uint64_t seq_tiles_bound(uint64_t n_tok, uint64_t n_seq, uint64_t group, uint64_t rows) {
+    return std::min<uint64_t>((n_tok * group + n_seq * (rows - 1)) / rows, n_tok * ((group + rows - 1) / rows));
+}
+
+// Row of position `pos` of a sequence in the key / value tensors: a row of the page pool (kv head
+// included) or of the packed prompts. Page numbers out of range give `none` and an error bit.
+constexpr uint32_t kNoRow = 0xffffffffu;
+__device__ __forceinline__ uint32_t seq_page(const SeqView &b, uint32_t seq, uint32_t idx) {
+    if (idx >= b.ld_pages) return kNoRow;
+    const int32_t pg = b.pages[(uint64_t)seq * b.ld_pages + idx];
+    if (pg < 0 || (uint32_t)pg >= b.n_pages) {
+        atomicOr(b.err, (uint32_t)ERR_BAD_ARG);
+        return kNoRow;
+    }
+    return (uint32_t)pg;
+}
+__device__ __forceinline__ uint32_t seq_kv_row(const SeqView &b, const SeqSpan &sp, uint32_t n_kv, uint32_t kvh,
+                                               uint32_t pos) {
+    if (!b.pages) return sp.first + pos;
+    const uint32_t pg = seq_page(b, sp.seq, pos >> b.page_shift);
+    if (pg == kNoRow) return kNoRow;
+    return ((pg * n_kv + kvh) << b.page_shift) + (pos & ((1u << b.page_shift) - 1));
+}
+
+// ---- elements ---------------------------------------------------------------------------------
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+// Two values rounded to E in one register (lo in the low half).
+template <typename E>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename E>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2 *>(&v)); }
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ---- thread-block clusters ---------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t smem, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// ---- attention over a batch of sequences --------------------------------------------------------
+struct SeqAttnParams {
+    SeqView b;
+    const void *q;
+    void *out;
+    const void *k, *v;          // for the row-by-row path
+    uint64_t ld_q, ld_out;      // elements between rows of q / out
+    uint64_t ld_kv, head_kv;    // elements between rows of k / v, and between a row's kv heads
+    uint32_t kv_rows;           // rows of k / v
+    uint32_t n_head, n_kv, group, hd, window, n_tiles, splits;
+    float softcap;
+};
+
+// One output row by one warp, from the formula, over the attended keys alone. The tiled kernels
+// multiply the probability 0 of a masked key with its value, which is NaN where that value is an
+// infinity or NaN; a row that comes out not finite is made again here, where masked keys are not
+// touched. An attended NaN or infinity stays what the formula makes of it.
+template <typename T, typename E>
+__device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan &sp, uint32_t t, uint32_t kvh, uint32_t g) {
+    const uint32_t lane = threadIdx.x & 31, head = kvh * p.group + g;
+    const int64_t pos = sp.pos(t);
+    const int64_t lo = p.window > 0 && pos + 1 > (int64_t)p.window ? pos + 1 - p.window : 0;
+    const T *q = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + t) * p.ld_q + (uint64_t)head * p.hd;
+    T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + t) * p.ld_out + (uint64_t)head * p.hd;
+    const uint32_t kvo = p.b.pages ? 0u : kvh * (uint32_t)p.head_kv;
+    float qv[8], o[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t d = lane + 32 * i;
+        qv[i] = d < p.hd ? to_f32(q[d]) : 0.0f;
+        o[i] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int64_t j = lo; j <= pos; j++) {
+        const uint32_t row = seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)j);
+        const E *kr = reinterpret_cast<const E *>(p.k) + (uint64_t)row * p.ld_kv + kvo;
+        const E *vr = reinterpret_cast<const E *>(p.v) + (uint64_t)row * p.ld_kv + kvo;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t d = lane + 32 * i;
+            if (d < p.hd && row != kNoRow) s = fmaf(qv[i], to_f32(kr[d]), s);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (p.softcap > 0.0f) s = p.softcap * tanhf(s / p.softcap);
+        const float mn = s > m ? s : m;
+        const float a = m == mn ? 1.0f : expf(m - mn), e = s == -INFINITY && mn == -INFINITY ? 0.0f : expf(s - mn);
+        m = mn;
+        l = l * a + e;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t d = lane + 32 * i;
+            if (d < p.hd) o[i] = o[i] * a + e * (row != kNoRow ? to_f32(vr[d]) : 0.0f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t d = lane + 32 * i;
+        if (d < p.hd) out[d] = from_f32<T>(lo > pos ? 0.0f : o[i] / l);
+    }
+}
+
+}  // namespace rcu

@@ -271,6 +271,29 @@ class CudaBackend:
                                                              out.size))
         return out
 
+    def score(self, tokens, pos: int, targets=None, top_k: int = 0) -> dict:
+        """Forward of tokens at pos.., scored on the device (rcu_backend_score): for each token's row
+        the log probability of targets[i] (-1: none), the entropy and the top_k most likely tokens,
+        without their logits coming to the host."""
+        tok = np.ascontiguousarray(tokens, dtype=np.uint32).reshape(-1)
+        n = tok.size
+        out = {"entropy": np.empty(n, dtype=np.float32), "top_ids": np.empty((n, top_k), dtype=np.int32),
+               "top_logprobs": np.empty((n, top_k), dtype=np.float32)}
+        tgt = None
+        if targets is not None:
+            tgt = np.ascontiguousarray(targets, dtype=np.int32).reshape(-1)
+            if tgt.size != n:
+                raise ValueError(f"{n} tokens need {n} targets, not {tgt.size}")
+            out["logprob"] = np.empty(n, dtype=np.float32)
+
+        def ptr(a):
+            return None if a is None or a.size == 0 else a.ctypes.data_as(C.c_void_p)
+
+        _check(self.ctx.ptr, _lib.load().rcu_backend_score(self.ptr, ptr(tok), n, pos, ptr(tgt), ptr(out.get("logprob")),
+                                                           ptr(out["entropy"]), top_k, ptr(out["top_ids"]),
+                                                           ptr(out["top_logprobs"])))
+        return out
+
     def forward_device(self, tokens_dev, n: int, pos: int, logits_dev, all_logits: bool = False) -> None:
         _check(self.ctx.ptr, _lib.load().rcu_backend_forward_device(self.ptr, C.c_void_p(_dptr(tokens_dev)), n, pos,
                                                                     int(all_logits), C.c_void_p(_dptr(logits_dev))))
