@@ -212,6 +212,7 @@ typedef struct rcu_seqs {
     const int32_t *pages; /* [n_seq][ld_pages]: position P of sequence i is in page pages[i][P / page_size] */
     uint64_t n_seq, n_tok, ld_pages;
     uint64_t max_len;     /* the longest len, 0 when unknown: shapes the launch, never the results */
+    uint64_t max_new;     /* the most new tokens of a sequence, 0 when unknown: the same */
 } rcu_seqs;
 /* Appends the new tokens' keys and values (post-RoPE keys; rows of n_head_kv * head_dim values of
  * ggml type F32, F16 or BF16, ld values apart, every row on a 16-byte boundary), rounded once to

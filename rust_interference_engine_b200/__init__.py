@@ -421,9 +421,10 @@ class SeqBatch:
 
     cu (n_seq + 1), len (n_seq) and pages (n_seq x width) are int32 CUDA tensors; the kernels read
     them when they run, so a captured graph replays with what they hold then. max_len (the longest
-    len, when the program knows it) shapes the launches, never the results."""
+    len) and max_new (the most new tokens of one sequence), when the program knows them, shape the
+    launches, never the results."""
 
-    def __init__(self, cu, len, pages, n_tok: int, max_len: int = 0):  # noqa: A002
+    def __init__(self, cu, len, pages, n_tok: int, max_len: int = 0, max_new: int = 0):  # noqa: A002
         for x, what, dims in ((cu, "cu", 1), (len, "len", 1), (pages, "pages", 2)):
             if str(x.dtype) != "torch.int32" or x.dim() != dims or not x.is_contiguous():
                 raise ValueError(f"{what}: expected a contiguous {dims}-dimensional int32 tensor")
@@ -432,11 +433,11 @@ class SeqBatch:
         n_seq = len.shape[0]
         if cu.shape[0] != n_seq + 1 or pages.shape[0] != n_seq:
             raise ValueError(f"{n_seq} sequences need {n_seq + 1} offsets and {n_seq} rows of pages")
-        if n_tok < 0 or max_len < 0:
-            raise ValueError("n_tok and max_len must not be negative")
+        if n_tok < 0 or max_len < 0 or max_new < 0:
+            raise ValueError("n_tok, max_len and max_new must not be negative")
         self.n_seq, self.n_tok, self.device = n_seq, n_tok, cu.get_device()
         self._keep = (cu, len, pages)
-        self._c = RcuSeqs(cu.data_ptr(), len.data_ptr(), pages.data_ptr(), n_seq, n_tok, pages.shape[1], max_len)
+        self._c = RcuSeqs(cu.data_ptr(), len.data_ptr(), pages.data_ptr(), n_seq, n_tok, pages.shape[1], max_len, max_new)
         self._ref = C.byref(self._c)
 
     def _on(self, ctx: Context):

@@ -88,7 +88,7 @@ class RcuJob(C.Structure):
 
 class RcuSeqs(C.Structure):
     _fields_ = [("cu", C.c_void_p), ("len", C.c_void_p), ("pages", C.c_void_p), ("n_seq", C.c_uint64),
-                ("n_tok", C.c_uint64), ("ld_pages", C.c_uint64), ("max_len", C.c_uint64)]
+                ("n_tok", C.c_uint64), ("ld_pages", C.c_uint64), ("max_len", C.c_uint64), ("max_new", C.c_uint64)]
 
 
 class RcuError(RuntimeError):

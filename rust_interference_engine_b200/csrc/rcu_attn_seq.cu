@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
     pdl_trigger();
     SeqSpan sp;
     uint32_t tile;
-    if (!seq_find_tile(p.b, p.group, kSqRows, ti, &sp, &tile)) return;  // the same for the whole cluster
+    if (!seq_find_tile(p.b, p.group, kSqRows, p.rows_lo, p.rows_hi, ti, &sp, &tile)) return;  // the same for the whole cluster
     if (lane == 0) {
         for (int s = 0; s < kSqStages; s++) mbar_init(&sm.full[warp][s], 1);
         fence_mbar_init();
@@ -400,64 +400,51 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
 // ---- host ---------------------------------------------------------------------------------------
 template <typename T, typename E, int HDP>
 static int launch_few(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv, SeqAttnParams p, uint64_t max_len) {
-    auto kern = k_attn_seq<T, E, HDP>;
     const size_t smem = sizeof(SqSmem<HDP>) + 1024;
-    RCU_CUDA_TRY(ctx, prefer_max_shared(reinterpret_cast<const void *>(kern)));
-    RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     // CTAs per tile: up to two for each SM in all, and at least 128 keys each
     const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + 16) : max_len;
-    uint32_t cs = 1;
     const uint32_t most = HDP == 256 ? 8 : kSqMaxCluster;  // 197 KB of shared memory each: eight SMs of a GPC are sure to be there
+    uint32_t cs = 1;
     while (cs < most && items * cs * 2 <= 2ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 128) cs *= 2;
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((uint32_t)(items * cs));
-    cfg.blockDim = dim3(kSqWarps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[2];
-    int na = 0;
-    if (cs > 1) {
-        attr[na].id = cudaLaunchAttributeClusterDimension;
-        attr[na].val.clusterDim.x = cs;
-        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
-        na++;
-    }
-    if (ctx->pdl) {
-        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[na].val.programmaticStreamSerializationAllowed = 1;
-        na++;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = na;
-    RCU_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, mk, mv, p));
-    return RCU_OK;
+    return launch_cluster_k(ctx, k_attn_seq<T, E, HDP>, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, mk, mv, p);
 }
 
 template <typename T, typename E>
-static int launch_seq(rcu_ctx *ctx, SeqAttnParams &p, const SeqKvDesc &kv, uint64_t max_len) {
-    const uint32_t hdp = p.hd <= 64 ? 64 : p.hd <= 128 ? 128 : 256;
+static int launch_few_hd(rcu_ctx *ctx, SeqAttnParams p, const SeqKvDesc &kv, uint64_t max_len) {
     CUtensorMap mk, mv;
-    const uint64_t heads = kv.pages ? 1 : p.n_kv;
-    for (int i = 0; i < 2; i++)
-        if (int st = make_map_3d(ctx, i ? &mv : &mk, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? kv.v : kv.k, p.hd, heads, kv.rows,
-                                 kv.head_stride * 2, kv.row_stride * 2, 64, 1, kSqKeys, CU_TENSOR_MAP_SWIZZLE_128B))
-            return st;
-    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kSqRows);
-    if (hdp == 64) return launch_few<T, E, 64>(ctx, mk, mv, p, max_len);
-    if (hdp == 128) return launch_few<T, E, 128>(ctx, mk, mv, p, max_len);
+    if (int st = seq_kv_maps(ctx, p, kv, kSqKeys, &mk, &mv)) return st;
+    // sequences of this class have fewer than rows_hi rows
+    const uint64_t each = (std::min<uint64_t>(p.rows_hi, (uint64_t)p.b.n_tok * p.group + 1) - 1 + kSqRows - 1) / kSqRows;
+    p.n_tiles = (uint32_t)std::min<uint64_t>(seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kSqRows), each * p.b.n_seq);
+    if (p.hd <= 64) return launch_few<T, E, 64>(ctx, mk, mv, p, max_len);
+    if (p.hd <= 128) return launch_few<T, E, 128>(ctx, mk, mv, p, max_len);
     return launch_few<T, E, 256>(ctx, mk, mv, p, max_len);
 }
 
-int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &params, int q_type, int kv_type, const SeqKvDesc &kv,
-                         uint64_t max_len) {
+static int launch_attention_few(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len) {
+    if (q_type == T_F32) return launch_few_hd<float, __half>(ctx, p, kv, max_len);
+    if (q_type == T_F16) return launch_few_hd<__half, __half>(ctx, p, kv, max_len);
+    return launch_few_hd<__nv_bfloat16, __nv_bfloat16>(ctx, p, kv, max_len);
+}
+
+int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &params, int q_type, const SeqKvDesc &kv, uint64_t max_len,
+                         uint64_t max_new) {
     SeqAttnParams p = params;
-    if (q_type == T_F32 && kv_type == T_F16) return launch_seq<float, __half>(ctx, p, kv, max_len);
-    if (q_type == T_F16 && kv_type == T_F16) return launch_seq<__half, __half>(ctx, p, kv, max_len);
-    if (q_type == T_BF16 && kv_type == T_BF16) return launch_seq<__nv_bfloat16, __nv_bfloat16>(ctx, p, kv, max_len);
-    return set_err(ctx, RCU_ERR_UNSUPPORTED, "attention: queries are f32 or f16 over f16 keys and values, or bf16 over bf16");
+    p.rows_lo = 0;
+    p.rows_hi = 0xffffffffu;
+    // The most query rows that a sequence may have. As many rows as sequences are taken for single
+    // tokens; what is there in fact only decides how fast the one launch is.
+    const uint64_t most = std::min<uint64_t>(max_new ? max_new : p.b.n_tok, p.b.n_tok) * p.group;
+    if (!attention_tile_ok(p.hd) || most < kTileMinRows || (!max_new && p.b.n_tok <= p.b.n_seq))
+        return launch_attention_few(ctx, p, q_type, kv, max_len);
+    if (p.b.n_seq == 1) return launch_attention_tile(ctx, p, q_type, kv, max_len);
+    p.rows_lo = kTileMinRows;
+    if (int st = launch_attention_tile(ctx, p, q_type, kv, max_len)) return st;
+    p.rows_lo = 0;
+    p.rows_hi = kTileMinRows;
+    return launch_attention_few(ctx, p, q_type, kv, max_len);
 }
 
 }  // namespace rcu

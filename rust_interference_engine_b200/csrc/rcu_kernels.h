@@ -126,8 +126,13 @@ struct SeqKvDesc {
     bool pages;
     uint64_t rows, row_stride, head_stride;  // strides in elements
 };
-int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, int kv_type, const SeqKvDesc &kv,
-                         uint64_t max_len);
+// (max_new too: 0 when unknown). q_type T_F32 or T_F16 over f16, or T_BF16 over bf16.
+int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,
+                         uint64_t max_new);
+// Its kernel for sequences of many query rows per KV head (rcu_attn_tile.cu), head_dim <= 128.
+constexpr uint32_t kTileMinRows = 64;
+bool attention_tile_ok(uint64_t hd);
+int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len);
 // log p of targets, entropy and the largest top_k of rows of logits (rcu_logprobs.cu).
 struct LogprobParams {
     const void *logits;

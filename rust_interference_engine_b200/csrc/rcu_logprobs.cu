@@ -293,34 +293,9 @@ __global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, 
 
 template <typename T>
 static int launch_lp(rcu_ctx *ctx, const LogprobParams &p) {
-    auto kern = k_logprobs<T>;
-    RCU_CUDA_TRY(ctx, prefer_max_shared(reinterpret_cast<const void *>(kern)));
-    RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(LpSmem)));
-    RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     uint32_t cs = 1;  // up to four CTAs for each SM, two steps of values for each
     while (cs < kLpMaxSplits && (uint64_t)p.rows * cs * 2 <= 4ull * ctx->num_sms && p.vocab >= (uint64_t)cs * 2 * kLpStep) cs *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.rows * cs);
-    cfg.blockDim = dim3(kLpThreads);
-    cfg.dynamicSmemBytes = sizeof(LpSmem);
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[2];
-    int na = 0;
-    if (cs > 1) {
-        attr[na].id = cudaLaunchAttributeClusterDimension;
-        attr[na].val.clusterDim.x = cs;
-        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
-        na++;
-    }
-    if (ctx->pdl) {
-        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[na].val.programmaticStreamSerializationAllowed = 1;
-        na++;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = na;
-    RCU_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, p, cs));
-    return RCU_OK;
+    return launch_cluster_k(ctx, k_logprobs<T>, p.rows * cs, kLpThreads, sizeof(LpSmem), cs, p, cs);
 }
 
 int launch_logprobs(rcu_ctx *ctx, const LogprobParams &p, int type) {

@@ -92,9 +92,10 @@ static int check_seqs(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s, SeqV
                  (uint32_t)pg->n_pages, pg->page_shift, ctx ? ctx->dev_err : nullptr};
     return RCU_OK;
 }
-static int check_heads(rcu_ctx *ctx, uint64_t n_head, uint64_t n_kv, uint64_t hd, uint64_t window, float softcap) {
+static int check_heads(rcu_ctx *ctx, uint64_t n_tok, uint64_t n_head, uint64_t n_kv, uint64_t hd, uint64_t window, float softcap) {
     if (n_head == 0 || n_kv == 0 || n_head % n_kv) return set_err(ctx, RCU_ERR_INVALID, "n_head not divisible by n_head_kv");
     if (hd == 0 || hd % 32 || hd > 256) return set_err(ctx, RCU_ERR_INVALID, "head_dim must be a multiple of 32 and <= 256");
+    if (n_tok * (n_head / n_kv) > 0x7fffff00ull) return set_err(ctx, RCU_ERR_INVALID, "batch too large");
     if (n_head > 4096) return set_err(ctx, RCU_ERR_INVALID, "more than 4096 query heads");
     if (window > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "window must be below 2^31 (0: none)");
     if (!(softcap < 3e38f)) return set_err(ctx, RCU_ERR_INVALID, "softcap must be finite (<= 0: none)");
@@ -199,7 +200,7 @@ int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s
     SeqAttnParams p{};
     if (!ctx || !q_dev || !out_dev) return set_err(ctx, RCU_ERR_INVALID, "null argument");
     if (int st = check_seqs(ctx, pg, seqs, &p.b)) return st;
-    if (int st = check_heads(ctx, n_head, pg->n_kv, pg->hd, window, softcap)) return st;
+    if (int st = check_heads(ctx, seqs->n_tok, n_head, pg->n_kv, pg->hd, window, softcap)) return st;
     if (type != T_F32 && type != T_F16) return set_err(ctx, RCU_ERR_UNSUPPORTED, "paged attention: queries are f32 or f16");
     if (int st = check_rows(ctx, "paged attention: q", q_dev, ld_q, n_head * pg->hd, (int)type)) return st;
     if (int st = check_rows(ctx, "paged attention: out", out_dev, ld_out, n_head * pg->hd, (int)type)) return st;
@@ -220,7 +221,7 @@ int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s
     const uint64_t cap = seqs->ld_pages * pg->page_size;
     DeviceGuard guard(ctx);
     const SeqKvDesc kv{pg->k, pg->v, true, p.kv_rows, pg->hd, pg->hd};
-    return launch_seq_attention(ctx, p, (int)type, T_F16, kv, seqs->max_len ? std::min(seqs->max_len, cap) : cap);
+    return launch_seq_attention(ctx, p, (int)type, kv, seqs->max_len ? std::min(seqs->max_len, cap) : cap, seqs->max_new);
     RCU_GUARD_END(ctx)
 }
 
@@ -231,7 +232,7 @@ int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, u
     RCU_GUARD_BEGIN
     if (!q_dev || !k_dev || !v_dev || !cu || !out_dev) return set_err(ctx, RCU_ERR_INVALID, "null argument");
     if (int st = check_batch(ctx, n_tok, n_seq)) return st;
-    if (int st = check_heads(ctx, n_head, n_head_kv, head_dim, window, softcap)) return st;
+    if (int st = check_heads(ctx, n_tok, n_head, n_head_kv, head_dim, window, softcap)) return st;
     if (!((q_type == T_F32 && kv_elem == T_F16) || (q_type == kv_elem && (q_type == T_F16 || q_type == T_BF16))))
         return set_err(ctx, RCU_ERR_UNSUPPORTED, "packed attention: queries are f32 or f16 over f16 keys and values, or bf16 over bf16");
     if (int st = check_rows(ctx, "packed attention: q", q_dev, ld_q, n_head * head_dim, (int)q_type)) return st;
@@ -258,7 +259,7 @@ int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, u
     p.softcap = softcap;
     DeviceGuard guard(ctx);
     const SeqKvDesc kv{k_dev, v_dev, false, n_tok, ld_kv, head_dim};
-    return launch_seq_attention(ctx, p, (int)q_type, (int)kv_elem, kv, max_len ? std::min(max_len, n_tok) : n_tok);
+    return launch_seq_attention(ctx, p, (int)q_type, kv, max_len ? std::min(max_len, n_tok) : n_tok, max_len);
     RCU_GUARD_END(ctx)
 }
 

@@ -11,7 +11,8 @@
 
 #include <algorithm>
 
-#include "rcu_internal.cuh"
+#include "rcu_kernels.h"
+#include "rcu_tc.cuh"
 
 namespace rcu {
 
@@ -47,17 +48,18 @@ __device__ __forceinline__ int64_t seq_len(const SeqView &b, uint32_t s, uint32_
     return min(max(l, (int64_t)0), cap);
 }
 
-// The sequence that holds work tile `ti` when sequence i takes ceil(n_new[i] * group / rows) tiles,
-// and the tile's number within it; false behind the last tile. One whole warp; the scan reads
-// 2 * n_seq words that stay in L1 / L2.
-__device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, uint32_t rows, uint32_t ti, SeqSpan *sp,
-                                              uint32_t *tile) {
+// The sequence that holds work tile `ti` when a sequence of n = n_new * group query rows takes
+// ceil(n / rows) tiles if rows_lo <= n < rows_hi and none otherwise, and the tile's number within
+// it; false behind the last tile. One whole warp; the scan reads 2 * n_seq words that stay in L1 / L2.
+__device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, uint32_t rows, uint32_t rows_lo,
+                                              uint32_t rows_hi, uint32_t ti, SeqSpan *sp, uint32_t *tile) {
     const uint32_t lane = threadIdx.x & 31;
     uint32_t base = 0;
     for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 32) {
         uint32_t first = 0, n = 0;
         if (s0 + lane < b.n_seq) n = seq_rows(b, s0 + lane, &first);
-        const uint32_t t = (uint32_t)(((uint64_t)n * group + rows - 1) / rows);
+        const uint32_t nr = n * group;  // below 2^31: the host checks n_tok * group
+        const uint32_t t = nr >= rows_lo && nr < rows_hi ? (nr + rows - 1) / rows : 0;
         uint32_t inc = t;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -173,6 +175,7 @@ struct SeqAttnParams {
     uint64_t ld_kv, head_kv;    // elements between rows of k / v, and between a row's kv heads
     uint32_t kv_rows;           // rows of k / v
     uint32_t n_head, n_kv, group, hd, window, n_tiles, splits;
+    uint32_t rows_lo, rows_hi;  // sequences of rows_lo <= n_new * group < rows_hi are this launch's
     float softcap;
 };
 
@@ -224,6 +227,47 @@ __device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan 
         const uint32_t d = lane + 32 * i;
         if (d < p.hd) out[d] = from_f32<T>(lo > pos ? 0.0f : o[i] / l);
     }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+// Tensor maps of k and v with boxes of `box` rows of 64 elements (128-byte swizzle).
+inline int seq_kv_maps(rcu_ctx *ctx, const SeqAttnParams &p, const SeqKvDesc &kv, uint32_t box, CUtensorMap *mk, CUtensorMap *mv) {
+    for (int i = 0; i < 2; i++)
+        if (int st = make_map_3d(ctx, i ? mv : mk, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? kv.v : kv.k, p.hd, kv.pages ? 1 : p.n_kv,
+                                 kv.rows, kv.head_stride * 2, kv.row_stride * 2, 64, 1, box, CU_TENSOR_MAP_SWIZZLE_128B))
+            return st;
+    return RCU_OK;
+}
+// Clusters of cs CTAs, programmatic dependent launch as launch_k.
+template <typename... KArgs, typename... Args>
+inline int launch_cluster_k(rcu_ctx *ctx, void (*kern)(KArgs...), uint32_t grid, uint32_t threads, size_t smem, uint32_t cs,
+                            const Args &...args) {
+    const void *fn = reinterpret_cast<const void *>(kern);
+    RCU_CUDA_TRY(ctx, prefer_max_shared(fn));
+    RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (cs > 8) RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (cs > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = cs;
+        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (ctx->pdl) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    RCU_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, args...));
+    return RCU_OK;
 }
 
 }  // namespace rcu
