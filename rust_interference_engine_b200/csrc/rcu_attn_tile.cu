@@ -35,6 +35,7 @@ constexpr int kTlThreads = 384;  // two softmax warpgroups; a third for the prod
 constexpr int kTlRegsSoftmax = 224, kTlRegsOther = 56;
 constexpr int kTlMaxCluster = 8;
 constexpr int kTlJoinWarps = 8;    // the softmax warps write the result
+constexpr int kTlPoly = 2;         // of 8 exponential pairs: on the FMA pipe, beside the special-function unit
 constexpr float kTlLazy = 8.0f, kTlShift = 7.0f;
 
 template <int HDP, bool SPLIT>
@@ -52,10 +53,16 @@ struct TlSmem {
     using C = TlCfg<HDP, SPLIT>;
     uint8_t data[C::kData];  // Q, then the ring; at the end O (f32, 16-byte chunks swizzled by row)
     float m[kTlRows], l[kTlRows];
-    uint64_t full[C::kStages], empty[C::kStages], q_full[2], s_full[2], p_full[2], done;
+    uint64_t full[C::kStages], empty[C::kStages], q_full[2], s_full[2], p_half[2], p_full[2], done;
     uint32_t tmem;
 };
 
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ void tl_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -119,6 +126,40 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return o;
 }
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// max over 32 values and mx (a tree, so that few steps wait for one another), NaN if one of them is
+__device__ __forceinline__ float tl_max32(const uint32_t (&s)[32], float mx) {
+    float c[11];
+#pragma unroll
+    for (int i = 0; i < 10; i++)
+        c[i] = max3_nan(__uint_as_float(s[3 * i]), __uint_as_float(s[3 * i + 1]), __uint_as_float(s[3 * i + 2]));
+    c[10] = max3_nan(__uint_as_float(s[30]), __uint_as_float(s[31]), mx);
+    const float d0 = max3_nan(c[0], c[1], c[2]), d1 = max3_nan(c[3], c[4], c[5]), d2 = max3_nan(c[6], c[7], c[8]);
+    return max3_nan(max3_nan(d0, d1, d2), c[9], c[10]);
+}
+// 2^x of two values on the FMA pipe, x <= 127 (below -126: 2^-126): x = n + f with n the nearest
+// whole number (from the addition of 1.5 * 2^23), 2^f by the polynomial of least relative error on
+// [-1/2, 1/2] (degree 4: 2.6e-6, degree 3: 7.5e-5; exchange algorithm in 64 bits), n into the exponent.
+template <int DEG>
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+    const float2 t = add2(x, make_float2(12582912.0f, 12582912.0f));
+    const float2 n = add2(t, make_float2(-12582912.0f, -12582912.0f));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    constexpr float c[2][5] = {{0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f, 0.0f},
+                               {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f, 0.009570102207362652f}};
+    float2 y = make_float2(c[DEG - 3][DEG], c[DEG - 3][DEG]);
+#pragma unroll
+    for (int i = DEG - 1; i >= 0; i--) y = fma2(y, f, make_float2(c[DEG - 3][i], c[DEG - 3][i]));
+    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
+    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
+    return y;
+}
+
 // Blocks [lo, hi) of keys that rows [r0, r1) of a sequence attend (r1 > r0).
 struct TlSpan {
     int32_t lo, hi;
@@ -140,7 +181,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
     constexpr int kChunks = HDP / 64;
     extern __shared__ __align__(1024) uint8_t tl_raw[];  // swizzled tiles start on 1024-byte boundaries
     S &sm = *reinterpret_cast<S *>(tl_raw);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = p.splits > 1 ? cluster_ctarank() : 0;
     const uint32_t item = blockIdx.x / p.splits, kvh = item % p.n_kv, ti = p.n_tiles - 1 - item / p.n_kv;
     pdl_wait();
@@ -165,7 +206,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-        for (int t = 0; t < 2; t++) mbar_init(&sm.q_full[t], 128), mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_full[t], 128);
+        for (int t = 0; t < 2; t++) mbar_init(&sm.q_full[t], 128), mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_half[t], 4), mbar_init(&sm.p_full[t], 4);
         mbar_init(&sm.done, 1);
         fence_mbar_init();
     }
@@ -208,59 +249,82 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         for (uint32_t i = it > C::kStages ? it - C::kStages : 0; i < it; i++)
             mbar_wait_sleep(&sm.full[i % C::kStages], (i / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
     } else if (warp == 9) {  // ---- MMA ----
-        if (lane == 0) {
-            constexpr uint32_t kFmt = std::is_same<E, __half>::value ? 0u : (1u << 7) | (1u << 10);
-            constexpr uint32_t kIdS = (1u << 4) | kFmt | ((uint32_t)(kTlBlk >> 3) << 17) | (8u << 24);
-            constexpr uint32_t kIdO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | (8u << 24);
-            bool ok = true;
-            for (int t = 0; t < (int)n_tiles && ok; t++) ok = mbar_wait_sleep(&sm.q_full[t], 0, p.b.err, ERR_TIMEOUT_FULL);
-            uint32_t np[2] = {0, 0};
-            for (int32_t j = j0; j <= j1 && ok; j++) {
-                const uint32_t ik = 2 * (uint32_t)(j - j0), iv = ik - 1;  // ring places of K(j), V(j - 1)
-                if (j > j0) ok = mbar_wait_bounded(&sm.full[iv % C::kStages], (iv / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
-                bool k_there = false;
+        // The whole warp walks the blocks and one elected lane issues: the loop's state is the same in
+        // every lane (taken from lane 0), so the descriptors stay in uniform registers. Issued from a
+        // branch of lane 0 alone, an MMA cost 107 cycles of moves into them, against 64 of work.
+        constexpr uint32_t kFmt = std::is_same<E, __half>::value ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t kIdS = (1u << 4) | kFmt | ((uint32_t)(kTlBlk >> 3) << 17) | (8u << 24);
+        constexpr uint32_t kIdO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | (8u << 24);
+        auto uni = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+        const int32_t n_blk = uni(j1 - j0), b0 = uni(jb[0] - j0), e0 = uni(je[0] - j0), b1 = uni(jb[1] - j0), e1 = uni(je[1] - j0);
+        const uint32_t tm = uni((int32_t)tmem);
+        const uint64_t dq = sw128_desc(sm.data), dk = sw128_desc(ring), dv = sw128_desc_mn(ring, kTlBlk * 128);
+        const bool elected = elect_one();
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
+            tc_fence_after();
+            return ok;
+        };
+        wait(&sm.q_full[0], 0);
+        if (uni((int32_t)n_tiles) > 1) wait(&sm.q_full[1], 0);
+        uint32_t np[2] = {0, 0};
+        uint32_t sk = 0, pk = 0, sv = 1, pv = 0;  // ring stage and parity of K(j), V(j - 1)
+        for (int32_t j = 0; j <= n_blk && ok; j++) {
+            const bool last = j == n_blk;
+            if (j > 0) wait(&sm.full[sv], pv);
+            if (!last) wait(&sm.full[sk], pk);
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const uint32_t ts = tmem + 128 * t, to = tmem + 256 + HDP * t;
-                    if (ok && j - 1 >= jb[t] && j - 1 < je[t]) {  // O_t += P_t V(j - 1)
-                        ok = mbar_wait_bounded(&sm.p_full[t], np[t]++ & 1, p.b.err, ERR_TIMEOUT_FULL);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint8_t *v = ring + (iv % C::kStages) * C::kStage;
+            for (int t = 0; t < 2; t++) {
+                const uint32_t ts = tm + 128 * t, to = tm + 256 + HDP * t;
+                const int32_t b = t ? b1 : b0, e = t ? e1 : e0;
+                if (j - 1 >= b && j - 1 < e && ok) {  // O_t += P_t V(j - 1)
+                    const uint64_t v = dv + sv * (C::kStage >> 4);
 #pragma unroll
-                        for (int kk = 0; kk < kTlBlk / 16; kk++) {
-                            const uint64_t b = sw128_desc_mn(v + 2048 * kk, kTlBlk * 128);
-                            const uint32_t a = ts + 32 * (kk >> 1) + 8 * (kk & 1);
-                            tl_mma_ts(to, a, b, kIdO, kk > 0 || (!kSplit && j - 1 > jb[t]));
-                            if constexpr (kSplit) tl_mma_ts(to, a + 16, b, kIdO, true);
+                    for (int half = 0; half < 2; half++) {  // keys 64 half .. 64 half + 63
+                        if (!wait(half ? &sm.p_full[t] : &sm.p_half[t], np[t] & 1)) break;
+                        if (elected) {
+#pragma unroll
+                            for (int kk = 4 * half; kk < 4 * half + 4; kk++) {
+                                const uint32_t a = ts + 32 * (kk >> 1) + 8 * (kk & 1);
+                                tl_mma_ts(to, a, v + (2048 >> 4) * kk, kIdO, kk > 0 || (!kSplit && j - 1 > b));
+                                if constexpr (kSplit) tl_mma_ts(to, a + 16, v + (2048 >> 4) * kk, kIdO, true);
+                            }
                         }
                     }
-                    if (t == 1 && j > j0) mma_commit(&sm.empty[iv % C::kStages]);
-                    if (j < j1 && ok && !k_there) {
-                        ok = mbar_wait_bounded(&sm.full[ik % C::kStages], (ik / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
-                        if (!ok) break;
-                        k_there = true;
-                        tc_fence_after();
-                    }
-                    if (j >= jb[t] && j < je[t]) {  // S_t = Q_t K(j)^T
-                        const uint8_t *k = ring + (ik % C::kStages) * C::kStage, *q = sm.data + t * C::kParts * C::kPart;
+                    np[t]++;
+                }
+                if (t == 1 && j > 0 && elected) mma_commit(&sm.empty[sv]);
+                if (j >= b && j < e && ok) {  // S_t = Q_t K(j)^T
+                    if (elected) {
+                        const uint64_t k = dk + sk * (C::kStage >> 4), q = dq + t * ((C::kParts * C::kPart) >> 4);
+                        if constexpr (kSplit) {
 #pragma unroll
-                        for (int kk = 0; kk < HDP / 16; kk++) {
-                            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                            if constexpr (kSplit) tl_mma_ss(ts, sw128_desc(q + C::kPart + off), sw128_desc(k + off), kIdS, kk > 0);
+                            for (int kk = 0; kk < HDP / 16; kk++) {
+                                const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+                                tl_mma_ss(ts, q + (C::kPart >> 4) + off, k + off, kIdS, kk > 0);
+                            }
                         }
 #pragma unroll
                         for (int kk = 0; kk < HDP / 16; kk++) {
-                            const uint32_t off = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-                            tl_mma_ss(ts, sw128_desc(q + off), sw128_desc(k + off), kIdS, kSplit || kk > 0);
+                            const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+                            tl_mma_ss(ts, q + off, k + off, kIdS, kSplit || kk > 0);
                         }
                         mma_commit(&sm.s_full[t]);
                     }
+                    __syncwarp();
                 }
-                if (ok && j < j1) mma_commit(&sm.empty[ik % C::kStages]);
             }
-            mma_commit(&sm.done);  // every MMA issued, on an early end too
+            if (!last && elected) mma_commit(&sm.empty[sk]);
+            // K and V blocks take turns in the ring
+            auto next = [](uint32_t &s, uint32_t &par) {
+                s += 2;
+                if (s >= (uint32_t)C::kStages) s -= C::kStages, par ^= 1;
+            };
+            if (j > 0) next(sv, pv);
+            next(sk, pk);
         }
+        if (elected) mma_commit(&sm.done);  // every MMA issued, on an early end too
         __syncwarp();
         mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN);
     } else if (warp < 8) {  // ---- softmax: thread r of tile t ----
@@ -352,14 +416,18 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                         if (32 * c + i > rhi || 32 * c + i < rlo) s[i] = 0xff800000u;
                 }
             };
-            auto pack = [&](int c, const uint32_t (&s)[32], float off, float2 &sum) {  // p, and its sum
+            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+            auto pack = [&](int c, const uint32_t (&s)[32], float off) {  // p, and its sum; the first 64 keys' P may go
                 uint32_t h[16], w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(cs, cs),
                                           make_float2(-off, -off));
-                    const float2 e = make_float2(ex2(x.x), ex2(x.y));
-                    sum = add2(sum, e);
+                    float2 e;
+                    if (!kSplit && i % 8 < kTlPoly) e = ex2_poly<std::is_same<E, __half>::value ? 4 : 3>(x);
+                    else e = make_float2(ex2(x.x), ex2(x.y));
+                    if (i & 1) sum1 = add2(sum1, e);
+                    else sum0 = add2(sum0, e);
                     h[i] = pack2<E>(e.x, e.y);
                     if constexpr (kSplit) {
                         const float2 f = unpack2<E>(h[i]);
@@ -368,19 +436,23 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 }
                 tl_tmem_st16(ts + 32 * c, h);
                 if constexpr (kSplit) tl_tmem_st16(ts + 32 * c + 16, w);
+                if (c & 1) {
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(c == 1 ? &sm.p_half[t] : &sm.p_full[t]);
+                }
             };
-            float2 sum = make_float2(0.0f, 0.0f);
+            float mx = -INFINITY;
             if constexpr (!kSplit) {
                 uint32_t s[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; c++) fetch(c, s[c]);
                 tmem_wait_ld();
-                float mx = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     shape(c, s[c]);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[c][i]));
+                    mx = tl_max32(s[c], mx);
                 }
                 mx *= cs;
                 const bool grow = mx > m + kTlLazy || (m == -INFINITY && mx > m);
@@ -403,17 +475,15 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 }
                 const float off = (m == -INFINITY ? 0.0f : m) - kTlShift;
 #pragma unroll
-                for (int c = 0; c < 4; c++) pack(c, s[c], off, sum);
+                for (int c = 0; c < 4; c++) pack(c, s[c], off);
             } else {
-                float mx = -INFINITY;
                 uint32_t s[32];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     fetch(c, s);
                     tmem_wait_ld();
                     shape(c, s);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
+                    mx = tl_max32(s, mx);
                 }
                 mx *= cs;
                 if (j > jb[t]) {  // add the last block's P V
@@ -426,7 +496,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                     }
                 }
                 if (__any_sync(0xffffffffu, mx > m)) {
-                    const float mn = fmaxf(m, mx);
+                    const float mn = mx > m ? mx : m;
                     const float a = mn == m ? 1.0f : ex2(m - mn);
                     m = mn;
                     l *= a;
@@ -439,13 +509,11 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                     fetch(c, s);
                     tmem_wait_ld();
                     shape(c, s);
-                    pack(c, s, off, sum);
+                    pack(c, s, off);
                 }
             }
-            l += sum.x + sum.y;
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sm.p_full[t]);
+            l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+            if (mx != mx) l = mx;  // a NaN among the scores (the polynomial does not carry it)
         }
         // every MMA has ended: Q and the ring are free for O
         ok = mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN) && ok;
