@@ -3,12 +3,14 @@
 //
 // A CTA takes 256 query rows (token, head of the group) of one sequence and KV head as two tiles of
 // 128 rows, and walks the attended keys in blocks of 128:
-//   * warp 8     producer: K and V blocks by tiled TMA (128-byte swizzle) into a ring of stages; a
+//   * warp 16    producer: K and V blocks by tiled TMA (128-byte swizzle) into a ring of stages; a
 //                page may be smaller than a block (one box per page) or larger;
-//   * warp 9     owns tensor memory; one thread issues S_t = Q_t K^T (M 128, N 128) and O_t += P_t V
+//   * warp 17    owns tensor memory; one thread issues S_t = Q_t K^T (M 128, N 128) and O_t += P_t V
 //                (P read from tensor memory, V in its own layout as an MN-major operand);
-//   * warps 0-3, 4-7  softmax of tile 0 / 1, one thread per query row: S out of tensor memory, mask,
-//                running maximum and sum in f32, P = 2^(s - m) back as packed 16-bit values over S.
+//   * warps 0-15 softmax, 8 for each tile: two threads share a query row, one for the first 64 keys of
+//                the block and one for the others: S out of tensor memory, mask, running maximum
+//                (the two exchange theirs) and sum in f32, P = 2^(s - m) back as packed 16-bit values
+//                over S, each half handed on by itself.
 // While one tile's warps are at their softmax, the tensor core works on the other tile.
 // 16-bit queries: O stays in tensor memory; it is rescaled only when a row's maximum has grown by
 // more than 2^kTlLazy since its last rescale (p then is at most 2^(kTlLazy + kTlShift)).
@@ -30,11 +32,11 @@ namespace rcu {
 
 constexpr int kTlRows = 256;       // query rows per CTA (two tiles)
 constexpr int kTlBlk = 128;        // keys per block
-constexpr int kTlThreads = 384;  // two softmax warpgroups; a third for the producer and the MMA issuer
-// registers a thread: the third warpgroup gives its own up (2 x 224 + 56 = 3 x 168, the launch's)
-constexpr int kTlRegsSoftmax = 224, kTlRegsOther = 56;
+constexpr int kTlSoftWarps = 16;
+constexpr int kTlThreads = 640;    // four softmax warpgroups; a fifth for the producer and the MMA issuer
+// registers a thread: the fifth warpgroup gives its own up (4 x 112 + 32 = 5 x 96, the launch's)
+constexpr int kTlRegsSoftmax = 112, kTlRegsOther = 32;
 constexpr int kTlMaxCluster = 8;
-constexpr int kTlJoinWarps = 8;    // the softmax warps write the result
 constexpr int kTlPoly = 2;         // of 8 exponential pairs: on the FMA pipe, beside the special-function unit
 constexpr float kTlLazy = 8.0f, kTlShift = 7.0f;
 
@@ -46,13 +48,13 @@ struct TlCfg {
     static constexpr int kStage = kTlBlk * HDP * 2;          // one K or V block
     static constexpr int kStages = HDP == 64 ? 8 : SPLIT ? 3 : 5;
     static constexpr int kData = kQ + kStages * kStage;
-    static_assert(kData >= kTlRows * HDP * 4, "the joined O overlays Q and the ring");
+    static_assert(kData >= kTlRows * HDP * 4 + 8 * kTlRows * 4, "the joined O and its weights overlay Q and the ring");
 };
 template <int HDP, bool SPLIT>
 struct TlSmem {
     using C = TlCfg<HDP, SPLIT>;
-    uint8_t data[C::kData];  // Q, then the ring; at the end O (f32, 16-byte chunks swizzled by row)
-    float m[kTlRows], l[kTlRows];
+    uint8_t data[C::kData];  // Q, then the ring; at the end O and its weights when a cluster joins
+    float mx[2][kTlRows];    // [half of the block's keys]: row maxima; at the end the row's m and l
     uint64_t full[C::kStages], empty[C::kStages], q_full[2], s_full[2], p_half[2], p_full[2], done;
     uint32_t tmem;
 };
@@ -95,15 +97,10 @@ __device__ __forceinline__ void tl_tmem_st16(uint32_t taddr, const uint32_t (&v)
         "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-__device__ __forceinline__ void tl_tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-        "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
-        "r"(v[31])
-        : "memory");
+__device__ __forceinline__ void tl_tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 // Two f32 lanes in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -131,15 +128,13 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// max over 32 values and mx (a tree, so that few steps wait for one another), NaN if one of them is
-__device__ __forceinline__ float tl_max32(const uint32_t (&s)[32], float mx) {
-    float c[11];
+// max of 16 values (a tree, so that few steps wait for one another), NaN if one of them is
+__device__ __forceinline__ float tl_max16(const uint32_t (&s)[16]) {
+    float c[5];
 #pragma unroll
-    for (int i = 0; i < 10; i++)
+    for (int i = 0; i < 5; i++)
         c[i] = max3_nan(__uint_as_float(s[3 * i]), __uint_as_float(s[3 * i + 1]), __uint_as_float(s[3 * i + 2]));
-    c[10] = max3_nan(__uint_as_float(s[30]), __uint_as_float(s[31]), mx);
-    const float d0 = max3_nan(c[0], c[1], c[2]), d1 = max3_nan(c[3], c[4], c[5]), d2 = max3_nan(c[6], c[7], c[8]);
-    return max3_nan(max3_nan(d0, d1, d2), c[9], c[10]);
+    return max3_nan(max3_nan(c[0], c[1], c[2]), max3_nan(c[3], c[4], __uint_as_float(s[15])), -INFINITY);
 }
 // 2^x of two values on the FMA pipe, x <= 127 (below -126: 2^-126): x = n + f with n the nearest
 // whole number (from the addition of 1.5 * 2^23), 2^f by the polynomial of least relative error on
@@ -206,21 +201,21 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-        for (int t = 0; t < 2; t++) mbar_init(&sm.q_full[t], 128), mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_half[t], 4), mbar_init(&sm.p_full[t], 4);
+        for (int t = 0; t < 2; t++) mbar_init(&sm.q_full[t], 256), mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_half[t], 4), mbar_init(&sm.p_full[t], 4);
         mbar_init(&sm.done, 1);
         fence_mbar_init();
     }
-    if (warp == 9) tmem_alloc<512>(&sm.tmem);
+    if (warp == kTlSoftWarps + 1) tmem_alloc<512>(&sm.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
     uint8_t *ring = sm.data + C::kQ;
 
-    if (warp >= 8) {
+    if (warp >= kTlSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTlRegsOther));
     }
-    if (warp == 8) {  // ---- producer ----
+    if (warp == kTlSoftWarps) {  // ---- producer ----
         const uint32_t box = p.b.pages ? min(1u << p.b.page_shift, (uint32_t)kTlBlk) : (uint32_t)kTlBlk;
         const uint32_t n_box = kTlBlk / box;  // boxes of rows per block (8 at most, pages of 16)
         const int64_t end = sp.pos((row0 + n_rows - 1) / p.group) + 1;
@@ -248,7 +243,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         // every copy has landed before this CTA goes on to its end
         for (uint32_t i = it > C::kStages ? it - C::kStages : 0; i < it; i++)
             mbar_wait_sleep(&sm.full[i % C::kStages], (i / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
-    } else if (warp == 9) {  // ---- MMA ----
+    } else if (warp == kTlSoftWarps + 1) {  // ---- MMA ----
         // The whole warp walks the blocks and one elected lane issues: the loop's state is the same in
         // every lane (taken from lane 0), so the descriptors stay in uniform registers. Issued from a
         // branch of lane 0 alone, an MMA cost 107 cycles of moves into them, against 64 of work.
@@ -262,7 +257,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         const bool elected = elect_one();
         bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
             tc_fence_after();
             return ok;
         };
@@ -286,9 +281,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                         if (elected) {
 #pragma unroll
                             for (int kk = 4 * half; kk < 4 * half + 4; kk++) {
-                                const uint32_t a = ts + 32 * (kk >> 1) + 8 * (kk & 1);
+                                const uint32_t a = ts + 16 * kk;
                                 tl_mma_ts(to, a, v + (2048 >> 4) * kk, kIdO, kk > 0 || (!kSplit && j - 1 > b));
-                                if constexpr (kSplit) tl_mma_ts(to, a + 16, v + (2048 >> 4) * kk, kIdO, true);
+                                if constexpr (kSplit) tl_mma_ts(to, a + 8, v + (2048 >> 4) * kk, kIdO, true);
                             }
                         }
                     }
@@ -327,54 +322,76 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         if (elected) mma_commit(&sm.done);  // every MMA issued, on an early end too
         __syncwarp();
         mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN);
-    } else if (warp < 8) {  // ---- softmax: thread r of tile t ----
+    } else if (warp < kTlSoftWarps) {  // ---- softmax: row r of tile t, keys 64 h .. 64 h + 63 of each block ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTlRegsSoftmax));
-        const uint32_t t = warp >> 2, r = threadIdx.x & 127;
-        const uint32_t lanes = (32 * (warp & 3)) << 16;  // this warp's TMEM lanes
-        const uint32_t ts = tmem + 128 * t + lanes, to = tmem + 256 + HDP * t + lanes;
-        const bool live = 128 * t + r < n_rows;
-        const uint32_t row = row0 + min(128 * t + r, n_rows - 1), tok = row / p.group;
+        const uint32_t t = warp >> 3, h = (warp >> 2) & 1, r = threadIdx.x & 127, tr = 128 * t + r;
+        const uint32_t pair = 1 + 4 * t + (warp & 3);    // barrier of the two warps that share these rows
+        const uint32_t lanes = (32 * (warp & 3)) << 16;  // their TMEM lanes
+        const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 256 + HDP * t + HDP / 2 * h + lanes;
+        const bool live = tr < n_rows;
+        const uint32_t row = row0 + min(tr, n_rows - 1), tok = row / p.group;
         const int64_t hi = live ? sp.pos(tok) : -1;
         const int64_t lo = p.window > 0 && hi + 1 > (int64_t)p.window ? hi + 1 - p.window : 0;
         float unscale = 1.0f;
-        if (t < n_tiles) {  // Q row into shared memory (K-major, 128-byte swizzle)
-            const T *src = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + tok) * p.ld_q +
-                           (uint64_t)(kvh * p.group + row % p.group) * p.hd;
-            uint8_t *q = sm.data + t * C::kParts * C::kPart + r * 128;
-            float scale = 1.0f;
+        if (t < n_tiles) {  // Q into shared memory (K-major, 128-byte swizzle), whole rows by neighbouring lanes
+            uint8_t *q = sm.data + t * C::kParts * C::kPart;
+            const uint32_t w8 = warp & 7;
+            auto source = [&](uint32_t i) {  // row i of the tile
+                const uint32_t rr = row0 + min(128 * t + i, n_rows - 1);
+                return reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + rr / p.group) * p.ld_q +
+                       (uint64_t)(kvh * p.group + rr % p.group) * p.hd;
+            };
             if constexpr (kSplit) {
-                float mx = 0.0f;
-                if (live)
-                    for (uint32_t c = 0; c < p.hd; c += 4) {
-                        const float4 x = *reinterpret_cast<const float4 *>(src + c);
-                        mx = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), mx);
-                    }
-                const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255), 2), 252) - 127;
-                scale = __uint_as_float((uint32_t)(127 - e) << 23);
-                unscale = __uint_as_float((uint32_t)(127 + e) << 23);
-            }
-#pragma unroll 4
-            for (int c = 0; c < HDP / 8; c++) {
-                uint8_t *d = q + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4);
-                const bool in = live && 8 * c < (int)p.hd;
-                if constexpr (kSplit) {
-                    float x[8] = {};
-                    if (in) {
-                        *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(src + 8 * c);
-                        *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(src + 8 * c + 4);
-                    }
-                    uint32_t h[4], w[4];
+                constexpr int kLanes = HDP / 4, kPer = 32 / kLanes;  // lanes of a row (4 values each), rows a warp and step
+                const uint32_t c4 = lane % kLanes, sub = lane / kLanes;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float a = x[2 * i] * scale, b = x[2 * i + 1] * scale;
-                        h[i] = pack2<E>(a, b);
-                        const float2 f = unpack2<E>(h[i]);
-                        w[i] = pack2<E>(a - f.x, b - f.y);
+                for (int g = 0; g < 16 / kPer; g += 4) {
+                    float4 x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t i = (w8 * (16 / kPer) + g + k) * kPer + sub;
+                        const bool in = 128 * t + i < n_rows && 4 * c4 < p.hd;
+                        x[k] = in ? *reinterpret_cast<const float4 *>(source(i) + 4 * c4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
-                    *reinterpret_cast<uint4 *>(d) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4 *>(d + C::kPart) = make_uint4(w[0], w[1], w[2], w[3]);
-                } else {
-                    *reinterpret_cast<uint4 *>(d) = in ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t i = (w8 * (16 / kPer) + g + k) * kPer + sub;
+                        float mx = fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+#pragma unroll
+                        for (int d = kLanes / 2; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                        // exponents at which both 2^e and 2^-e are normal numbers
+                        const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255), 2), 252) - 127;
+                        const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
+                        if (c4 == 0) sm.mx[0][128 * t + i] = __uint_as_float((uint32_t)(127 + e) << 23);
+                        uint32_t u[2], w[2];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const float a = (j ? x[k].z : x[k].x) * scale, b = (j ? x[k].w : x[k].y) * scale;
+                            u[j] = pack2<E>(a, b);
+                            const float2 f = unpack2<E>(u[j]);
+                            w[j] = pack2<E>(a - f.x, b - f.y);
+                        }
+                        const uint32_t c = c4 >> 1;
+                        uint8_t *d = q + (c >> 3) * (128 * 128) + i * 128 + (((c & 7) ^ (i & 7)) << 4) + 8 * (c4 & 1);
+                        *reinterpret_cast<uint2 *>(d) = make_uint2(u[0], u[1]);
+                        *reinterpret_cast<uint2 *>(d + C::kPart) = make_uint2(w[0], w[1]);
+                    }
+                }
+                named_bar_sync(9 + t, 256);
+                unscale = sm.mx[0][tr];
+            } else {
+                constexpr int kLanes = HDP / 8, kPer = 32 / kLanes, kIt = 16 / kPer;
+                const uint32_t c = lane % kLanes, sub = lane / kLanes;
+                uint4 x[kIt];
+#pragma unroll
+                for (int k = 0; k < kIt; k++) {
+                    const uint32_t i = (w8 * kIt + k) * kPer + sub;
+                    x[k] = 128 * t + i < n_rows && 8 * c < p.hd ? *reinterpret_cast<const uint4 *>(source(i) + 8 * c) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int k = 0; k < kIt; k++) {
+                    const uint32_t i = (w8 * kIt + k) * kPer + sub;
+                    *reinterpret_cast<uint4 *>(q + (c >> 3) * (128 * 128) + i * 128 + (((c & 7) ^ (i & 7)) << 4)) = x[k];
                 }
             }
             fence_async_smem();
@@ -389,219 +406,283 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         }
         const float cs = p.softcap > 0.0f ? 1.0f : unscale * kLog2e;
         float m = -INFINITY, l = 0.0f;  // m in units of log2, as last rescaled to
-        float o[kSplit ? HDP : 1];
+        float o[kSplit ? HDP / 2 : 1];  // f32: this thread's half of O's columns, without the last block
         if constexpr (kSplit) {
 #pragma unroll
-            for (int i = 0; i < HDP; i++) o[i] = 0.0f;
+            for (int i = 0; i < HDP / 2; i++) o[i] = 0.0f;
         }
         bool ok = true;
         for (int32_t j = jb[t]; j < je[t]; j++) {
-            ok = mbar_wait_bounded(&sm.s_full[t], (j - jb[t]) & 1, p.b.err, ERR_TIMEOUT_FULL);
+            ok = mbar_wait_spin(&sm.s_full[t], (j - jb[t]) & 1, p.b.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
-            const int64_t key0 = (int64_t)j * kTlBlk;
-            const bool part = key0 < all_lo || key0 + kTlBlk - 1 > all_hi;
-            const int32_t rlo = (int32_t)max(lo - key0, (int64_t)0), rhi = (int32_t)max(min(hi - key0, (int64_t)kTlBlk), (int64_t)-1);
-            // one block's columns 32 c .. 32 c + 31 of this row: softcapped, masked
-            auto fetch = [&](int c, uint32_t (&s)[32]) { tmem_ld32(ts + 32 * c, s); };
-            auto shape = [&](int c, uint32_t (&s)[32]) {
+            const int64_t key0 = (int64_t)j * kTlBlk + 64 * h;
+            const bool part = key0 < all_lo || key0 + 63 > all_hi;
+            const int32_t rlo = (int32_t)max(lo - key0, (int64_t)0), rhi = (int32_t)max(min(hi - key0, (int64_t)64), (int64_t)-1);
+            // 16 scores of chunk c: softcapped (then in units of log2), masked
+            auto shape = [&](int c, uint32_t (&s)[16]) {
                 if (p.softcap > 0.0f) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
+                    for (int i = 0; i < 16; i++)
                         s[i] = __float_as_uint(p.softcap * kLog2e * tanhf(__uint_as_float(s[i]) * unscale / p.softcap));
                 }
                 if (part) {
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (32 * c + i > rhi || 32 * c + i < rlo) s[i] = 0xff800000u;
+                    for (int i = 0; i < 16; i++)
+                        if (16 * c + i > rhi || 16 * c + i < rlo) s[i] = 0xff800000u;
                 }
             };
-            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-            auto pack = [&](int c, const uint32_t (&s)[32], float off) {  // p, and its sum; the first 64 keys' P may go
-                uint32_t h[16], w[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(cs, cs),
-                                          make_float2(-off, -off));
-                    float2 e;
-                    if (!kSplit && i % 8 < kTlPoly) e = ex2_poly<std::is_same<E, __half>::value ? 4 : 3>(x);
-                    else e = make_float2(ex2(x.x), ex2(x.y));
-                    if (i & 1) sum1 = add2(sum1, e);
-                    else sum0 = add2(sum0, e);
-                    h[i] = pack2<E>(e.x, e.y);
-                    if constexpr (kSplit) {
-                        const float2 f = unpack2<E>(h[i]);
-                        w[i] = pack2<E>(e.x - f.x, e.y - f.y);
-                    }
-                }
-                tl_tmem_st16(ts + 32 * c, h);
-                if constexpr (kSplit) tl_tmem_st16(ts + 32 * c + 16, w);
-                if (c & 1) {
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(c == 1 ? &sm.p_half[t] : &sm.p_full[t]);
-                }
-            };
+            const bool shaped = part || p.softcap > 0.0f;
+            // 16-bit: the scores stay in registers. f32: they are read again after the maximum, since
+            // the registers hold O.
+            uint32_t s[kSplit ? 2 : 4][16];
             float mx = -INFINITY;
             if constexpr (!kSplit) {
-                uint32_t s[4][32];
 #pragma unroll
-                for (int c = 0; c < 4; c++) fetch(c, s[c]);
+                for (int c = 0; c < 4; c++) tmem_ld16(ts + 16 * c, s[c]);
                 tmem_wait_ld();
+                if (shaped) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    shape(c, s[c]);
-                    mx = tl_max32(s[c], mx);
+                    for (int c = 0; c < 4; c++) shape(c, s[c]);
                 }
-                mx *= cs;
-                const bool grow = mx > m + kTlLazy || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float mn = grow ? mx : m;
-                    const float a = mn == m ? 1.0f : ex2(m - mn);
-                    m = mn;
-                    l *= a;
-                    if (j > jb[t]) {  // the S that was waited for comes after the last P V
-#pragma unroll
-                        for (int c = 0; c < HDP / 32; c++) {
-                            uint32_t v[32];
-                            tmem_ld32(to + 32 * c, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-                            tl_tmem_st32(to + 32 * c, v);
-                        }
-                    }
-                }
-                const float off = (m == -INFINITY ? 0.0f : m) - kTlShift;
-#pragma unroll
-                for (int c = 0; c < 4; c++) pack(c, s[c], off);
+                mx = max3_nan(max3_nan(tl_max16(s[0]), tl_max16(s[1]), tl_max16(s[2])), tl_max16(s[3]), -INFINITY);
             } else {
-                uint32_t s[32];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    fetch(c, s);
+                for (int c = 0; c < 4; c += 2) {
+                    tmem_ld16(ts + 16 * c, s[0]);
+                    tmem_ld16(ts + 16 * c + 16, s[1]);
                     tmem_wait_ld();
-                    shape(c, s);
-                    mx = tl_max32(s, mx);
+                    if (shaped) shape(c, s[0]), shape(c + 1, s[1]);
+                    mx = max3_nan(mx, tl_max16(s[0]), tl_max16(s[1]));
                 }
-                mx *= cs;
+            }
+            sm.mx[h][tr] = mx;
+            named_bar_sync(pair, 64);
+            mx = max3_nan(mx, sm.mx[h ^ 1][tr], -INFINITY) * cs;
+            const bool grow = kSplit ? mx > m : mx > m + kTlLazy || (m == -INFINITY && mx > m);
+            if constexpr (kSplit) {
                 if (j > jb[t]) {  // add the last block's P V
 #pragma unroll
                     for (int c = 0; c < HDP / 32; c++) {
-                        tmem_ld32(to + 32 * c, s);
+                        uint32_t v[16];
+                        tmem_ld16(to + 16 * c, v);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[32 * c + i] += __uint_as_float(s[i]);
+                        for (int i = 0; i < 16; i++) o[16 * c + i] += __uint_as_float(v[i]);
                     }
                 }
-                if (__any_sync(0xffffffffu, mx > m)) {
-                    const float mn = mx > m ? mx : m;
-                    const float a = mn == m ? 1.0f : ex2(m - mn);
-                    m = mn;
-                    l *= a;
+            }
+            if (__any_sync(0xffffffffu, grow)) {  // the same for the other warp of these rows
+                const float mn = grow ? mx : m;
+                const float a = mn == m ? 1.0f : ex2(m - mn);
+                m = mn;
+                l *= a;
+                if constexpr (kSplit) {
 #pragma unroll
-                    for (int i = 0; i < HDP; i++) o[i] *= a;
-                }
-                const float off = (m == -INFINITY ? 0.0f : m) - kTlShift;
+                    for (int i = 0; i < HDP / 2; i++) o[i] *= a;
+                } else if (j > jb[t]) {  // the S that was waited for comes after the last P V
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    fetch(c, s);
-                    tmem_wait_ld();
-                    shape(c, s);
-                    pack(c, s, off);
+                    for (int c = 0; c < HDP / 32; c++) {
+                        uint32_t v[16];
+                        tmem_ld16(to + 16 * c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
+                        tl_tmem_st16(to + 16 * c, v);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    named_bar_sync(pair, 64);  // neither half's P goes on before all of O is rescaled
+                    tc_fence_after();
                 }
             }
+            const float off = (m == -INFINITY ? 0.0f : m) - kTlShift;
+            float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t (&x)[16] = s[kSplit ? 0 : c];
+                if constexpr (kSplit) {
+                    tmem_ld16(ts + 16 * c, x);
+                    tmem_wait_ld();
+                    if (shaped) shape(c, x);
+                }
+                uint32_t u[8], w[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float2 y = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])),
+                                          make_float2(cs, cs), make_float2(-off, -off));
+                    float2 e;
+                    if (!kSplit && i < kTlPoly) e = ex2_poly<std::is_same<E, __half>::value ? 4 : 3>(y);
+                    else e = make_float2(ex2(y.x), ex2(y.y));
+                    if (i & 1) sum1 = add2(sum1, e);
+                    else sum0 = add2(sum0, e);
+                    u[i] = pack2<E>(e.x, e.y);
+                    if constexpr (kSplit) {
+                        const float2 f = unpack2<E>(u[i]);
+                        w[i] = pack2<E>(e.x - f.x, e.y - f.y);
+                    }
+                }
+                tl_tmem_st8(ts + 16 * c, u);
+                if constexpr (kSplit) tl_tmem_st8(ts + 16 * c + 8, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h ? &sm.p_full[t] : &sm.p_half[t]);
             l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
             if (mx != mx) l = mx;  // a NaN among the scores (the polynomial does not carry it)
         }
-        // every MMA has ended: Q and the ring are free for O
-        ok = mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN) && ok;
+        // every MMA has ended
+        ok = mbar_wait_spin(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN) && ok;
         tc_fence_after();
+        const bool any = je[t] > jb[t] && ok;
         if (t < n_tiles) {
-            float *orow = reinterpret_cast<float *>(sm.data) + (128 * t + r) * HDP;
-            constexpr uint32_t kMask = HDP / 4 - 1;
-            const bool any = je[t] > jb[t] && ok;
+            if (h == 1) sm.mx[1][tr] = l;
+            named_bar_sync(pair, 64);
+            if (h == 0) l += sm.mx[1][tr], sm.mx[0][tr] = m, sm.mx[1][tr] = l;
+            named_bar_sync(pair, 64);
+            l = sm.mx[1][tr];
+        }
+        // this thread's half of O's columns, 16 at a time
+        auto columns = [&](int c, float (&x)[16]) {
+            uint32_t v[16];
+            if (any) {
+                tmem_ld16(to + 16 * c, v);
+                tmem_wait_ld();
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                x[i] = any ? __uint_as_float(v[i]) : 0.0f;
+                if constexpr (kSplit) x[i] += o[16 * c + i];
+            }
+        };
+        if (p.splits == 1) {
+            // rounded rows through shared memory (16-byte chunks swizzled by row), so that neighbouring
+            // lanes store neighbouring bytes: a row of each lane's own cost 9000 cycles against 2000
+            if (t < n_tiles) {
+                constexpr int kRowB = HDP * sizeof(T), kVec = kRowB / 16, kPer = 16 / sizeof(T);  // bytes, chunks, values a chunk
+                uint8_t *st = sm.data + t * 128 * kRowB;
+                const float inv = 1.0f / l;
+                bool fine = true;
+#pragma unroll
+                for (int c = 0; c < HDP / 32; c++) {
+                    float x[16];
+                    columns(c, x);
+                    alignas(16) T y[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float f = x[i] * inv;
+                        fine = fine && isfinite(f);
+                        y[i] = from_f32<T>(f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < (int)sizeof(T); i++)
+                        *reinterpret_cast<uint4 *>(st + r * kRowB + ((((kVec / 2 * h) + (int)sizeof(T) * c + i) ^ (r & 7)) << 4)) =
+                            reinterpret_cast<const uint4 *>(y)[i];
+                }
+                tc_fence_before();
+                named_bar_sync(9 + t, 256);
+                constexpr int kLanes = kVec < 32 ? kVec : 32, kRows = 32 / kLanes;
+                const uint32_t ch = lane % kLanes;
+#pragma unroll 4
+                for (uint32_t k = 0; k < 16 / kRows; k++) {
+                    const uint32_t i = ((warp & 7) * (16 / kRows) + k) * kRows + lane / kLanes;
+                    if (128 * t + i >= n_rows || ch * kPer >= p.hd) continue;
+                    const uint32_t rr = row0 + 128 * t + i;
+                    T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + rr / p.group) * p.ld_out +
+                              (uint64_t)(kvh * p.group + rr % p.group) * p.hd;
+                    *reinterpret_cast<uint4 *>(orow + ch * kPer) = *reinterpret_cast<const uint4 *>(st + i * kRowB + ((ch ^ (i & 7)) << 4));
+                }
+                uint32_t bad = __ballot_sync(0xffffffffu, live && !fine);
+                named_bar_sync(9 + t, 256);  // every row is written: now the ones that are not finite again
+                while (bad) {
+                    const int b = __ffs((int)bad) - 1;
+                    bad &= bad - 1;
+                    const uint32_t rr = row0 + 128 * t + 32 * (warp & 3) + b;
+                    seq_attn_row<T, E>(p, sp, rr / p.group, kvh, rr % p.group);
+                }
+            }
+            tc_fence_before();
+            __syncthreads();  // tensor memory may go
+            return;
+        }
+        // ---- joined over the cluster: every CTA's O in its shared memory (16-byte chunks swizzled by
+        // row, over Q and the ring), then the rows are shared out over the cluster's warps ----
+        if (t < n_tiles) {
+            float *orow = reinterpret_cast<float *>(sm.data) + tr * HDP;
 #pragma unroll
             for (int c = 0; c < HDP / 32; c++) {
-                uint32_t v[32];
-                if (any) {
-                    tmem_ld32(to + 32 * c, v);
-                    tmem_wait_ld();
-                }
+                float x[16];
+                columns(c, x);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float x[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        x[k] = any ? __uint_as_float(v[4 * i + k]) : 0.0f;
-                        if constexpr (kSplit) x[k] += o[32 * c + 4 * i + k];
-                    }
-                    *reinterpret_cast<float4 *>(orow + (((8 * c + i) ^ (r & kMask)) << 2)) = make_float4(x[0], x[1], x[2], x[3]);
-                }
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(orow + (((HDP / 8 * h + 4 * c + i) ^ (r & (HDP / 4 - 1))) << 2)) =
+                        make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
-            sm.m[128 * t + r] = m;
-            sm.l[128 * t + r] = l;
         }
         tc_fence_before();
-        if (p.splits > 1) cluster_sync_all();
-        else __syncthreads();
-        // ---- rows of the result over the warps of the cluster ----
-        constexpr int VE = HDP / 32;  // values a lane
-        for (uint32_t r = rank * kTlJoinWarps + warp; r < n_rows; r += p.splits * kTlJoinWarps) {
-            float acc[VE] = {};
-            float L;
-            // lane's values: 16-byte chunk lane * VE / 4, swizzled by the row
-            const uint32_t ch = (lane * VE / 4) ^ (r & (HDP / 4 - 1)), at = r * HDP * 4 + ch * 16 + (lane * VE % 4) * 4;
-            if (p.splits == 1) {
-                L = sm.l[r];
-    #pragma unroll
-                for (int i = 0; i < VE; i++) acc[i] = *reinterpret_cast<const float *>(sm.data + at + 4 * i);
-            } else {
-                const uint32_t am = smem_u32(&sm.m[r]), al = smem_u32(&sm.l[r]), ao = smem_u32(sm.data) + at;
-                const float mc = lane < p.splits ? ld_cluster_f32(cluster_addr(am, lane)) : -INFINITY;
-                const float lc = lane < p.splits ? ld_cluster_f32(cluster_addr(al, lane)) : 0.0f;
-                float M = mc;
-    #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-                const float ac = mc == -INFINITY ? 0.0f : ex2(mc - M);
-                L = ac * lc;
-    #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
-                for (uint32_t c = 0; c < p.splits; c++) {
-                    const float w = __shfl_sync(0xffffffffu, ac, c);
-                    if (w == 0.0f) continue;
-                    const uint32_t a = cluster_addr(ao, c);
-    #pragma unroll
-                    for (int i = 0; i < VE; i++) acc[i] = fmaf(w, ld_cluster_f32(a + 4 * i), acc[i]);
-                }
+        cluster_sync_all();
+        // weight of each CTA's part of row i: 2^(m_c - max m) / sum_c l_c 2^(m_c - max m)
+        float *wt = reinterpret_cast<float *>(sm.data + kTlRows * HDP * 4);
+        if (threadIdx.x < n_rows) {
+            const uint32_t i = threadIdx.x, am = smem_u32(&sm.mx[0][i]), al = smem_u32(&sm.mx[1][i]);
+            float mc[kTlMaxCluster], lc[kTlMaxCluster], M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kTlMaxCluster; c++) {
+                mc[c] = c < (int)p.splits ? ld_cluster_f32(cluster_addr(am, c)) : -INFINITY;
+                lc[c] = c < (int)p.splits ? ld_cluster_f32(cluster_addr(al, c)) : 0.0f;
+                M = fmaxf(M, mc[c]);
             }
-            const uint32_t rr = row0 + r, tk = rr / p.group, gq = rr % p.group, d0 = lane * VE;
+#pragma unroll
+            for (int c = 0; c < kTlMaxCluster; c++) {
+                mc[c] = mc[c] == -INFINITY ? 0.0f : ex2(mc[c] - M);
+                if (c < (int)p.splits) L = fmaf(mc[c], lc[c], L);
+            }
+            const float inv = 1.0f / L;
+#pragma unroll
+            for (int c = 0; c < kTlMaxCluster; c++)
+                if (c < (int)p.splits) wt[c * kTlRows + i] = mc[c] * inv;
+            if (!isfinite(inv)) wt[i] = __uint_as_float(0x7fffffffu);  // no keys, or a NaN: the row is made again
+        }
+        named_bar_sync(15, kTlSoftWarps * 32);
+        constexpr int kVec = HDP / 4;  // 16-byte chunks of a row
+        const uint32_t step = p.splits * kTlSoftWarps * 32 / kVec, ch = lane % kVec;
+#pragma unroll 2
+        for (uint32_t i = (rank * kTlSoftWarps + warp) * (32 / kVec) + lane / kVec; i - lane / kVec < n_rows; i += step) {
+            const bool in = i < n_rows;
+            const uint32_t a = smem_u32(sm.data) + (in ? i * HDP * 4 + ((ch ^ (i & (kVec - 1))) << 4) : 0);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int c = 0; c < kTlMaxCluster; c++) {
+                if (c >= (int)p.splits || !in) continue;
+                const float w = wt[c * kTlRows + i];
+                const float4 x = ld_cluster_f32x4(cluster_addr(a, c));
+                if (w != 0.0f) v = make_float4(fmaf(w, x.x, v.x), fmaf(w, x.y, v.y), fmaf(w, x.z, v.z), fmaf(w, x.w, v.w));
+            }
+            const uint32_t rr = row0 + (in ? i : 0), tk = rr / p.group, gq = rr % p.group;
             T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + tk) * p.ld_out + (uint64_t)(kvh * p.group + gq) * p.hd;
-            bool fine = true;
-            if (d0 < p.hd) {
-                alignas(16) T v[VE];
-    #pragma unroll
-                for (int i = 0; i < VE; i++) {
-                    const float x = acc[i] / L;
-                    fine = fine && isfinite(x);
-                    v[i] = from_f32<T>(x);
-                }
-                if constexpr (VE * sizeof(T) == 16) *reinterpret_cast<uint4 *>(orow + d0) = *reinterpret_cast<const uint4 *>(v);
-                else if constexpr (VE * sizeof(T) == 8) *reinterpret_cast<uint2 *>(orow + d0) = *reinterpret_cast<const uint2 *>(v);
-                else *reinterpret_cast<uint32_t *>(orow + d0) = *reinterpret_cast<const uint32_t *>(v);
+            const bool fine = !in || 4 * ch >= p.hd || (isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+            if (in && 4 * ch < p.hd) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(orow + 4 * ch) = v;
+                else *reinterpret_cast<uint2 *>(orow + 4 * ch) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
             }
-            if (!__all_sync(0xffffffffu, fine)) {
+            uint32_t bad = __ballot_sync(0xffffffffu, !fine);
+            if (bad) {
                 __syncwarp();
-                seq_attn_row<T, E>(p, sp, tk, kvh, gq);
+#pragma unroll 1
+                for (int k = 0; k < 32 / kVec; k++)
+                    if (bad >> (k * kVec) & (kVec == 32 ? 0xffffffffu : (1u << kVec) - 1)) {
+                        const uint32_t rb = __shfl_sync(0xffffffffu, rr, k * kVec);
+                        seq_attn_row<T, E>(p, sp, rb / p.group, kvh, rb % p.group);
+                    }
             }
         }
-        if (p.splits > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory
+        cluster_sync_all();  // no CTA leaves while another reads its shared memory
         return;
     }
     if (p.splits > 1) cluster_sync_all();
     else __syncthreads();
-    if (warp == 9) {
+    if (warp == kTlSoftWarps + 1) {
         tc_fence_after();
         tmem_free<512>(tmem);
     }

@@ -145,6 +145,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// A bounded wait that looks at the clock once in 256 polls only: reading it takes longer than the
+// phase change it would notice.
+__device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+    if (mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255) == 0) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > kWaitLimitNs) {
+                atomicOr(err, code);
+                return false;
+            }
+        }
+    }
+}
+
 // ---- thread-block clusters ---------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
@@ -158,6 +176,11 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t smem, uint32_t rank) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(rank));
     return a;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t a) {
     float v;
