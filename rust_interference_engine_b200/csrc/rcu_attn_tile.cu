@@ -330,8 +330,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 256 + HDP * t + HDP / 2 * h + lanes;
         const bool live = tr < n_rows;
         const uint32_t row = row0 + min(tr, n_rows - 1), tok = row / p.group;
-        const int64_t hi = live ? sp.pos(tok) : -1;
-        const int64_t lo = p.window > 0 && hi + 1 > (int64_t)p.window ? hi + 1 - p.window : 0;
+        // positions stay below 2^31
+        const int32_t hi = live ? (int32_t)sp.pos(tok) : -1;
+        const int32_t lo = p.window > 0 ? max(hi - (int32_t)p.window + 1, 0) : 0;
         float unscale = 1.0f;
         if (t < n_tiles) {  // Q into shared memory (K-major, 128-byte swizzle), whole rows by neighbouring lanes
             uint8_t *q = sm.data + t * C::kParts * C::kPart;
@@ -398,11 +399,11 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             mbar_arrive(&sm.q_full[t]);
         }
         // keys that every live row of the tile attends: blocks inside need no mask
-        int64_t all_hi = -1, all_lo = 0;
+        int32_t all_hi = -1, all_lo = 0;
         if (t < n_tiles) {
-            const int64_t last = sp.pos((min(row0 + n_rows, row0 + 128 * t + 128) - 1) / p.group);
-            all_hi = sp.pos((row0 + 128 * t) / p.group);
-            all_lo = p.window > 0 && last + 1 > (int64_t)p.window ? last + 1 - p.window : 0;
+            const int32_t last = (int32_t)sp.pos((min(row0 + n_rows, row0 + 128 * t + 128) - 1) / p.group);
+            all_hi = (int32_t)sp.pos((row0 + 128 * t) / p.group);
+            all_lo = p.window > 0 ? max(last - (int32_t)p.window + 1, 0) : 0;
         }
         const float cs = p.softcap > 0.0f ? 1.0f : unscale * kLog2e;
         float m = -INFINITY, l = 0.0f;  // m in units of log2, as last rescaled to
@@ -416,9 +417,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             ok = mbar_wait_spin(&sm.s_full[t], (j - jb[t]) & 1, p.b.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
-            const int64_t key0 = (int64_t)j * kTlBlk + 64 * h;
+            const int32_t key0 = j * kTlBlk + 64 * (int32_t)h;
             const bool part = key0 < all_lo || key0 + 63 > all_hi;
-            const int32_t rlo = (int32_t)max(lo - key0, (int64_t)0), rhi = (int32_t)max(min(hi - key0, (int64_t)64), (int64_t)-1);
+            const int32_t rlo = lo - key0, rhi = hi - key0;
             // 16 scores of chunk c: softcapped (then in units of log2), masked
             auto shape = [&](int c, uint32_t (&s)[16]) {
                 if (p.softcap > 0.0f) {

@@ -145,20 +145,20 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// A bounded wait that looks at the clock once in 256 polls only: reading it takes longer than the
-// phase change it would notice.
+// A bounded wait whose polls suspend the thread until the phase changes (at most 0.1 ms each), and
+// that reads the clock, which takes longer than a wake-up, only between them.
 __device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
-    if (mbar_try_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255) == 0) {
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > kWaitLimitNs) {
-                atomicOr(err, code);
-                return false;
-            }
+    constexpr uint32_t kHintNs = 100000;
+    if (mbar_try_wait_hint(bar, parity, kHintNs)) return true;
+    if (mbar_try_wait_hint(bar, parity, kHintNs)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 16; i++)
+            if (mbar_try_wait_hint(bar, parity, kHintNs)) return true;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(err, code);
+            return false;
         }
     }
 }
