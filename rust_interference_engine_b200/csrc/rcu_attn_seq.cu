@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
     pdl_trigger();
     SeqSpan sp;
     uint32_t tile;
-    if (!seq_find_tile(p.b, p.group, kSqRows, p.rows_lo, p.rows_hi, ti, &sp, &tile)) return;  // the same for the whole cluster
+    if (!seq_find_tile(p.b, p.group, kSqRows, ti, &sp, &tile)) return;  // the same for the whole cluster
     if (lane == 0) {
         for (int s = 0; s < kSqStages; s++) mbar_init(&sm.full[warp][s], 1);
         fence_mbar_init();
@@ -415,9 +415,7 @@ template <typename T, typename E>
 static int launch_few_hd(rcu_ctx *ctx, SeqAttnParams p, const SeqKvDesc &kv, uint64_t max_len) {
     CUtensorMap mk, mv;
     if (int st = seq_kv_maps(ctx, p, kv, kSqKeys, &mk, &mv)) return st;
-    // sequences of this class have fewer than rows_hi rows
-    const uint64_t each = (std::min<uint64_t>(p.rows_hi, (uint64_t)p.b.n_tok * p.group + 1) - 1 + kSqRows - 1) / kSqRows;
-    p.n_tiles = (uint32_t)std::min<uint64_t>(seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kSqRows), each * p.b.n_seq);
+    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kSqRows);
     if (p.hd <= 64) return launch_few<T, E, 64>(ctx, mk, mv, p, max_len);
     if (p.hd <= 128) return launch_few<T, E, 128>(ctx, mk, mv, p, max_len);
     return launch_few<T, E, 256>(ctx, mk, mv, p, max_len);
@@ -429,22 +427,17 @@ static int launch_attention_few(rcu_ctx *ctx, const SeqAttnParams &p, int q_type
     return launch_few_hd<__nv_bfloat16, __nv_bfloat16>(ctx, p, kv, max_len);
 }
 
-int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &params, int q_type, const SeqKvDesc &kv, uint64_t max_len,
+int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,
                          uint64_t max_new) {
-    SeqAttnParams p = params;
-    p.rows_lo = 0;
-    p.rows_hi = 0xffffffffu;
-    // The most query rows that a sequence may have. As many rows as sequences are taken for single
-    // tokens; what is there in fact only decides how fast the one launch is.
+    // The most query rows that a sequence may have in one KV head. As many new rows as sequences are
+    // taken for single tokens; what is there in fact decides only how fast the launch is. One kernel
+    // takes the whole batch: in a mixed one the single tokens ride along with the chunks (two chunks
+    // of 333 tokens beside 14 single ones: 64 us for the chunks alone and 62 us for the single
+    // tokens in a launch of their own).
     const uint64_t most = std::min<uint64_t>(max_new ? max_new : p.b.n_tok, p.b.n_tok) * p.group;
     if (!attention_tile_ok(p.hd) || most < kTileMinRows || (!max_new && p.b.n_tok <= p.b.n_seq))
         return launch_attention_few(ctx, p, q_type, kv, max_len);
-    if (p.b.n_seq == 1) return launch_attention_tile(ctx, p, q_type, kv, max_len);
-    p.rows_lo = kTileMinRows;
-    if (int st = launch_attention_tile(ctx, p, q_type, kv, max_len)) return st;
-    p.rows_lo = 0;
-    p.rows_hi = kTileMinRows;
-    return launch_attention_few(ctx, p, q_type, kv, max_len);
+    return launch_attention_tile(ctx, p, q_type, kv, max_len);
 }
 
 }  // namespace rcu

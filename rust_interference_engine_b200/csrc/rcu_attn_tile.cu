@@ -55,7 +55,7 @@ struct TlSmem {
     using C = TlCfg<HDP, SPLIT>;
     uint8_t data[C::kData];  // Q, then the ring; at the end O and its weights when a cluster joins
     float mx[2][kTlRows];    // [half of the block's keys]: row maxima; at the end the row's m and l
-    uint64_t full[C::kStages], empty[C::kStages], q_full[2], s_full[2], p_half[2], p_full[2], done;
+    uint64_t full[C::kStages], empty[C::kStages], s_full[2], p_half[2], p_full[2], o_done[2], done;
     uint32_t tmem;
 };
 
@@ -179,11 +179,26 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = p.splits > 1 ? cluster_ctarank() : 0;
     const uint32_t item = blockIdx.x / p.splits, kvh = item % p.n_kv, ti = p.n_tiles - 1 - item / p.n_kv;
+    // what needs no input first: tensor memory, and the barriers by the warp that uses them at once
+    if (warp == kTlSoftWarps + 1) tmem_alloc<512>(&sm.tmem);
+    if (warp == kTlSoftWarps) {
+        if (lane == 0) {
+            for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
+            for (int t = 0; t < 2; t++)
+                mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_half[t], 4), mbar_init(&sm.p_full[t], 4), mbar_init(&sm.o_done[t], 1);
+            mbar_init(&sm.done, 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+    }
     pdl_wait();
     pdl_trigger();
     SeqSpan sp;
     uint32_t tile;
-    if (!seq_find_tile(p.b, p.group, kTlRows, p.rows_lo, p.rows_hi, ti, &sp, &tile)) return;  // the same for the whole cluster
+    if (!seq_find_tile(p.b, p.group, kTlRows, ti, &sp, &tile)) {  // the same for the whole cluster
+        if (warp == kTlSoftWarps + 1) tmem_free<512>(sm.tmem);
+        return;
+    }
     const uint32_t row0 = tile * kTlRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kTlRows);
     const uint32_t n_tiles = n_rows > 128 ? 2 : 1;
     // this CTA's part of the blocks, and each tile's part of those
@@ -199,141 +214,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             jb[t] = min(max(s.lo, j0), j1), je[t] = max(min(s.hi, j1), jb[t]);
         }
     }
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-        for (int t = 0; t < 2; t++) mbar_init(&sm.q_full[t], 256), mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_half[t], 4), mbar_init(&sm.p_full[t], 4);
-        mbar_init(&sm.done, 1);
-        fence_mbar_init();
-    }
-    if (warp == kTlSoftWarps + 1) tmem_alloc<512>(&sm.tmem);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = sm.tmem;
     uint8_t *ring = sm.data + C::kQ;
-
-    if (warp >= kTlSoftWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTlRegsOther));
-    }
-    if (warp == kTlSoftWarps) {  // ---- producer ----
-        const uint32_t box = p.b.pages ? min(1u << p.b.page_shift, (uint32_t)kTlBlk) : (uint32_t)kTlBlk;
-        const uint32_t n_box = kTlBlk / box;  // boxes of rows per block (8 at most, pages of 16)
-        const int64_t end = sp.pos((row0 + n_rows - 1) / p.group) + 1;
-        uint32_t it = 0;
-        bool ok = true;
-        for (int32_t j = j0; j < j1 && ok; j++) {
-            // lane l < n_box * kChunks brings box l % n_box of 64-element chunk l / n_box
-            const uint32_t bx = lane % n_box, ch = lane / n_box;
-            const int64_t pos = (int64_t)j * kTlBlk + bx * box;
-            uint32_t row = p.kv_rows;  // behind the tensor: zeros
-            if (ch < kChunks && pos < end) row = min(seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)pos), p.kv_rows);
-#pragma unroll
-            for (int kv = 0; kv < 2; kv++, it++) {
-                const uint32_t s = it % C::kStages, n = it / C::kStages;
-                if (n > 0) ok = ok && mbar_wait_sleep(&sm.empty[s], (n - 1) & 1, p.b.err, ERR_TIMEOUT_EMPTY);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(&sm.full[s], C::kStage);
-                __syncwarp();
-                if (ch < kChunks)
-                    tma_load_3d(ring + s * C::kStage + ch * (kTlBlk * 128) + bx * box * 128, kv ? &mv : &mk, 64 * ch,
-                                p.b.pages ? 0 : (int)kvh, (int)row, &sm.full[s]);
-            }
-        }
-        // every copy has landed before this CTA goes on to its end
-        for (uint32_t i = it > C::kStages ? it - C::kStages : 0; i < it; i++)
-            mbar_wait_sleep(&sm.full[i % C::kStages], (i / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
-    } else if (warp == kTlSoftWarps + 1) {  // ---- MMA ----
-        // The whole warp walks the blocks and one elected lane issues: the loop's state is the same in
-        // every lane (taken from lane 0), so the descriptors stay in uniform registers. Issued from a
-        // branch of lane 0 alone, an MMA cost 107 cycles of moves into them, against 64 of work.
-        constexpr uint32_t kFmt = std::is_same<E, __half>::value ? 0u : (1u << 7) | (1u << 10);
-        constexpr uint32_t kIdS = (1u << 4) | kFmt | ((uint32_t)(kTlBlk >> 3) << 17) | (8u << 24);
-        constexpr uint32_t kIdO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | (8u << 24);
-        auto uni = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
-        const int32_t n_blk = uni(j1 - j0), b0 = uni(jb[0] - j0), e0 = uni(je[0] - j0), b1 = uni(jb[1] - j0), e1 = uni(je[1] - j0);
-        const uint32_t tm = uni((int32_t)tmem);
-        const uint64_t dq = sw128_desc(sm.data), dk = sw128_desc(ring), dv = sw128_desc_mn(ring, kTlBlk * 128);
-        const bool elected = elect_one();
-        bool ok = true;
-        auto wait = [&](uint64_t *bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
-            tc_fence_after();
-            return ok;
-        };
-        wait(&sm.q_full[0], 0);
-        if (uni((int32_t)n_tiles) > 1) wait(&sm.q_full[1], 0);
-        uint32_t np[2] = {0, 0};
-        uint32_t sk = 0, pk = 0, sv = 1, pv = 0;  // ring stage and parity of K(j), V(j - 1)
-        for (int32_t j = 0; j <= n_blk && ok; j++) {
-            const bool last = j == n_blk;
-            if (j > 0) wait(&sm.full[sv], pv);
-            if (!last) wait(&sm.full[sk], pk);
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t ts = tm + 128 * t, to = tm + 256 + HDP * t;
-                const int32_t b = t ? b1 : b0, e = t ? e1 : e0;
-                if (j - 1 >= b && j - 1 < e && ok) {  // O_t += P_t V(j - 1)
-                    const uint64_t v = dv + sv * (C::kStage >> 4);
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {  // keys 64 half .. 64 half + 63
-                        if (!wait(half ? &sm.p_full[t] : &sm.p_half[t], np[t] & 1)) break;
-                        if (elected) {
-#pragma unroll
-                            for (int kk = 4 * half; kk < 4 * half + 4; kk++) {
-                                const uint32_t a = ts + 16 * kk;
-                                tl_mma_ts(to, a, v + (2048 >> 4) * kk, kIdO, kk > 0 || (!kSplit && j - 1 > b));
-                                if constexpr (kSplit) tl_mma_ts(to, a + 8, v + (2048 >> 4) * kk, kIdO, true);
-                            }
-                        }
-                    }
-                    np[t]++;
-                }
-                if (t == 1 && j > 0 && elected) mma_commit(&sm.empty[sv]);
-                if (j >= b && j < e && ok) {  // S_t = Q_t K(j)^T
-                    if (elected) {
-                        const uint64_t k = dk + sk * (C::kStage >> 4), q = dq + t * ((C::kParts * C::kPart) >> 4);
-                        if constexpr (kSplit) {
-#pragma unroll
-                            for (int kk = 0; kk < HDP / 16; kk++) {
-                                const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-                                tl_mma_ss(ts, q + (C::kPart >> 4) + off, k + off, kIdS, kk > 0);
-                            }
-                        }
-#pragma unroll
-                        for (int kk = 0; kk < HDP / 16; kk++) {
-                            const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-                            tl_mma_ss(ts, q + off, k + off, kIdS, kSplit || kk > 0);
-                        }
-                        mma_commit(&sm.s_full[t]);
-                    }
-                    __syncwarp();
-                }
-            }
-            if (!last && elected) mma_commit(&sm.empty[sk]);
-            // K and V blocks take turns in the ring
-            auto next = [](uint32_t &s, uint32_t &par) {
-                s += 2;
-                if (s >= (uint32_t)C::kStages) s -= C::kStages, par ^= 1;
-            };
-            if (j > 0) next(sv, pv);
-            next(sk, pk);
-        }
-        if (elected) mma_commit(&sm.done);  // every MMA issued, on an early end too
-        __syncwarp();
-        mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN);
-    } else if (warp < kTlSoftWarps) {  // ---- softmax: row r of tile t, keys 64 h .. 64 h + 63 of each block ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTlRegsSoftmax));
-        const uint32_t t = warp >> 3, h = (warp >> 2) & 1, r = threadIdx.x & 127, tr = 128 * t + r;
-        const uint32_t pair = 1 + 4 * t + (warp & 3);    // barrier of the two warps that share these rows
-        const uint32_t lanes = (32 * (warp & 3)) << 16;  // their TMEM lanes
-        const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 256 + HDP * t + HDP / 2 * h + lanes;
-        const bool live = tr < n_rows;
-        const uint32_t row = row0 + min(tr, n_rows - 1), tok = row / p.group;
-        // positions stay below 2^31
-        const int32_t hi = live ? (int32_t)sp.pos(tok) : -1;
-        const int32_t lo = p.window > 0 ? max(hi - (int32_t)p.window + 1, 0) : 0;
-        float unscale = 1.0f;
+    if (warp < kTlSoftWarps) {
+        const uint32_t t = warp >> 3;
         if (t < n_tiles) {  // Q into shared memory (K-major, 128-byte swizzle), whole rows by neighbouring lanes
             uint8_t *q = sm.data + t * C::kParts * C::kPart;
             const uint32_t w8 = warp & 7;
@@ -378,8 +261,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                         *reinterpret_cast<uint2 *>(d + C::kPart) = make_uint2(w[0], w[1]);
                     }
                 }
-                named_bar_sync(9 + t, 256);
-                unscale = sm.mx[0][tr];
             } else {
                 constexpr int kLanes = HDP / 8, kPer = 32 / kLanes, kIt = 16 / kPer;
                 const uint32_t c = lane % kLanes, sub = lane / kLanes;
@@ -396,14 +277,153 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 }
             }
             fence_async_smem();
-            mbar_arrive(&sm.q_full[t]);
         }
+    }
+    uint32_t tmem = 0;
+    auto meet = [&]() {  // Q, the barriers and tensor memory are there
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = sm.tmem;
+    };
+    if (warp != kTlSoftWarps) meet();  // the producer has its copies on their way first
+    if (warp >= kTlSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTlRegsOther));
+    }
+    if (warp == kTlSoftWarps) {  // ---- producer ----
+        bool met = false;
+        const uint32_t box = p.b.pages ? min(1u << p.b.page_shift, (uint32_t)kTlBlk) : (uint32_t)kTlBlk;
+        const uint32_t n_box = kTlBlk / box;  // boxes of rows per block (8 at most, pages of 16)
+        const int64_t end = sp.pos((row0 + n_rows - 1) / p.group) + 1;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int32_t j = j0; j < j1 && ok; j++) {
+            if (it + 2 > C::kStages && !met) met = true, meet();
+            // lane l < n_box * kChunks brings box l % n_box of 64-element chunk l / n_box
+            const uint32_t bx = lane % n_box, ch = lane / n_box;
+            const int64_t pos = (int64_t)j * kTlBlk + bx * box;
+            uint32_t row = p.kv_rows;  // behind the tensor: zeros
+            if (ch < kChunks && pos < end) row = min(seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)pos), p.kv_rows);
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++, it++) {
+                const uint32_t s = it % C::kStages, n = it / C::kStages;
+                if (n > 0) ok = ok && mbar_wait_sleep(&sm.empty[s], (n - 1) & 1, p.b.err, ERR_TIMEOUT_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&sm.full[s], C::kStage);
+                __syncwarp();
+                if (ch < kChunks)
+                    tma_load_3d(ring + s * C::kStage + ch * (kTlBlk * 128) + bx * box * 128, kv ? &mv : &mk, 64 * ch,
+                                p.b.pages ? 0 : (int)kvh, (int)row, &sm.full[s]);
+            }
+        }
+        if (!met) meet();
+        // every copy has landed before this CTA goes on to its end
+        for (uint32_t i = it > C::kStages ? it - C::kStages : 0; i < it; i++)
+            mbar_wait_sleep(&sm.full[i % C::kStages], (i / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
+    } else if (warp == kTlSoftWarps + 1) {  // ---- MMA ----
+        // The whole warp walks the blocks and one elected lane issues: the loop's state is the same in
+        // every lane (taken from lane 0), so the descriptors stay in uniform registers. Issued from a
+        // branch of lane 0 alone, an MMA cost 107 cycles of moves into them, against 64 of work.
+        constexpr uint32_t kFmt = std::is_same<E, __half>::value ? 0u : (1u << 7) | (1u << 10);
+        constexpr uint32_t kIdS = (1u << 4) | kFmt | ((uint32_t)(kTlBlk >> 3) << 17) | (8u << 24);
+        constexpr uint32_t kIdO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | (8u << 24);
+        auto uni = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+        const int32_t n_blk = uni(j1 - j0), b0 = uni(jb[0] - j0), e0 = uni(je[0] - j0), b1 = uni(jb[1] - j0), e1 = uni(je[1] - j0);
+        const uint32_t tm = uni((int32_t)tmem);
+        const uint64_t dq = sw128_desc(sm.data), dk = sw128_desc(ring), dv = sw128_desc_mn(ring, kTlBlk * 128);
+        const bool elected = elect_one();
+        bool ok = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
+            tc_fence_after();
+            return ok;
+        };
+        uint32_t np[2] = {0, 0};
+        uint32_t sk = 0, pk = 0, sv = 1, pv = 0;  // ring stage and parity of K(j), V(j - 1)
+        for (int32_t j = 0; j <= n_blk && ok; j++) {
+            const bool last = j == n_blk;
+            if (j > 0) wait(&sm.full[sv], pv);
+            if (!last) wait(&sm.full[sk], pk);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const uint32_t ts = tm + 128 * t, to = tm + 256 + HDP * t;
+                const int32_t b = t ? b1 : b0, e = t ? e1 : e0;
+                if (j - 1 >= b && j - 1 < e && ok) {  // O_t += P_t V(j - 1)
+                    const uint64_t v = dv + sv * (C::kStage >> 4);
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {  // keys 64 half .. 64 half + 63
+                        if (!wait(half ? &sm.p_full[t] : &sm.p_half[t], np[t] & 1)) break;
+                        if (elected) {
+#pragma unroll
+                            for (int kk = 4 * half; kk < 4 * half + 4; kk++) {
+                                const uint32_t a = ts + 16 * kk;
+                                tl_mma_ts(to, a, v + (2048 >> 4) * kk, kIdO, kk > 0 || (!kSplit && j - 1 > b));
+                                if constexpr (kSplit) tl_mma_ts(to, a + 8, v + (2048 >> 4) * kk, kIdO, true);
+                            }
+                        }
+                    }
+                    np[t]++;
+                    if (j == e && elected) mma_commit(&sm.o_done[t]);
+                }
+                if (t == 1 && j > 0 && elected) mma_commit(&sm.empty[sv]);
+                if (j >= b && j < e && ok) {  // S_t = Q_t K(j)^T
+                    if (elected) {
+                        const uint64_t k = dk + sk * (C::kStage >> 4), q = dq + t * ((C::kParts * C::kPart) >> 4);
+                        if constexpr (kSplit) {
+#pragma unroll
+                            for (int kk = 0; kk < HDP / 16; kk++) {
+                                const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+                                tl_mma_ss(ts, q + (C::kPart >> 4) + off, k + off, kIdS, kk > 0);
+                            }
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < HDP / 16; kk++) {
+                            const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+                            tl_mma_ss(ts, q + off, k + off, kIdS, kSplit || kk > 0);
+                        }
+                        mma_commit(&sm.s_full[t]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (!last && elected) mma_commit(&sm.empty[sk]);
+            // K and V blocks take turns in the ring
+            auto next = [](uint32_t &s, uint32_t &par) {
+                s += 2;
+                if (s >= (uint32_t)C::kStages) s -= C::kStages, par ^= 1;
+            };
+            if (j > 0) next(sv, pv);
+            next(sk, pk);
+        }
+        if (elected) {
+            if (!ok) mma_commit(&sm.o_done[0]), mma_commit(&sm.o_done[1]);
+            mma_commit(&sm.done);  // every MMA issued, on an early end too
+        }
+        __syncwarp();
+        mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN);
+    } else if (warp < kTlSoftWarps) {  // ---- softmax: row r of tile t, keys 64 h .. 64 h + 63 of each block ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTlRegsSoftmax));
+        const uint32_t t = warp >> 3, h = (warp >> 2) & 1, r = threadIdx.x & 127, tr = 128 * t + r;
+        const uint32_t pair = 1 + 4 * t + (warp & 3);    // barrier of the two warps that share these rows
+        const uint32_t lanes = (32 * (warp & 3)) << 16;  // their TMEM lanes
+        const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 256 + HDP * t + HDP / 2 * h + lanes;
+        const bool live = tr < n_rows;
+        const uint32_t row = row0 + min(tr, n_rows - 1), tok = row / p.group;
+        // positions stay below 2^31
+        const int32_t hi = live ? (int32_t)sp.pos(tok) : -1;
+        const int32_t lo = p.window > 0 ? max(hi - (int32_t)p.window + 1, 0) : 0;
         // keys that every live row of the tile attends: blocks inside need no mask
         int32_t all_hi = -1, all_lo = 0;
         if (t < n_tiles) {
             const int32_t last = (int32_t)sp.pos((min(row0 + n_rows, row0 + 128 * t + 128) - 1) / p.group);
             all_hi = (int32_t)sp.pos((row0 + 128 * t) / p.group);
             all_lo = p.window > 0 ? max(last - (int32_t)p.window + 1, 0) : 0;
+        }
+        float unscale = 1.0f;
+        if constexpr (kSplit) {
+            unscale = t < n_tiles ? sm.mx[0][tr] : 1.0f;
+            named_bar_sync(pair, 64);  // both have read it before either writes a maximum there
         }
         const float cs = p.softcap > 0.0f ? 1.0f : unscale * kLog2e;
         float m = -INFINITY, l = 0.0f;  // m in units of log2, as last rescaled to
@@ -533,10 +553,11 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
             if (mx != mx) l = mx;  // a NaN among the scores (the polynomial does not carry it)
         }
-        // every MMA has ended
-        ok = mbar_wait_spin(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN) && ok;
+        // this tile's MMAs have ended (when a cluster joins, every MMA: O goes over Q and the ring)
+        const bool own = je[t] > jb[t];
+        if (p.splits > 1 || own) ok = mbar_wait_spin(p.splits > 1 ? &sm.done : &sm.o_done[t], 0, p.b.err, ERR_TIMEOUT_DRAIN) && ok;
         tc_fence_after();
-        const bool any = je[t] > jb[t] && ok;
+        const bool any = own && ok;
         if (t < n_tiles) {
             if (h == 1) sm.mx[1][tr] = l;
             named_bar_sync(pair, 64);
@@ -558,8 +579,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             }
         };
         if (p.splits == 1) {
-            // rounded rows through shared memory (16-byte chunks swizzled by row), so that neighbouring
-            // lanes store neighbouring bytes: a row of each lane's own cost 9000 cycles against 2000
+            // rounded rows through shared memory (over the tile's own Q, 16-byte chunks swizzled by row),
+            // so that neighbouring lanes store neighbouring bytes: a row of each lane's own cost 9000
+            // cycles a CTA against 3000
             if (t < n_tiles) {
                 constexpr int kRowB = HDP * sizeof(T), kVec = kRowB / 16, kPer = 16 / sizeof(T);  // bytes, chunks, values a chunk
                 uint8_t *st = sm.data + t * 128 * kRowB;
@@ -710,10 +732,7 @@ static int launch_tile_hd(rcu_ctx *ctx, SeqAttnParams &p, const SeqKvDesc &kv, u
     CUtensorMap mk, mv;
     const uint32_t box = kv.pages ? std::min<uint32_t>(1u << p.b.page_shift, kTlBlk) : kTlBlk;
     if (int st = seq_kv_maps(ctx, p, kv, box, &mk, &mv)) return st;
-    // sequences of this class have at least rows_lo rows (or there is one class only)
-    const uint64_t rows = (uint64_t)p.b.n_tok * p.group;
-    p.n_tiles = (uint32_t)std::min<uint64_t>(seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kTlRows),
-                                             rows / kTlRows + rows / std::max(1u, p.rows_lo) + 1);
+    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kTlRows);
     return p.hd <= 64 ? launch_tile<T, E, 64>(ctx, mk, mv, p, max_len) : launch_tile<T, E, 128>(ctx, mk, mv, p, max_len);
 }
 

@@ -48,18 +48,17 @@ __device__ __forceinline__ int64_t seq_len(const SeqView &b, uint32_t s, uint32_
     return min(max(l, (int64_t)0), cap);
 }
 
-// The sequence that holds work tile `ti` when a sequence of n = n_new * group query rows takes
-// ceil(n / rows) tiles if rows_lo <= n < rows_hi and none otherwise, and the tile's number within
-// it; false behind the last tile. One whole warp; the scan reads 2 * n_seq words that stay in L1 / L2.
-__device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, uint32_t rows, uint32_t rows_lo,
-                                              uint32_t rows_hi, uint32_t ti, SeqSpan *sp, uint32_t *tile) {
+// The sequence that holds work tile `ti` when each sequence takes ceil(n_new * group / rows) tiles,
+// and the tile's number within it; false behind the last tile. One whole warp; the scan reads
+// 2 * n_seq words that stay in L1 / L2.
+__device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, uint32_t rows, uint32_t ti, SeqSpan *sp,
+                                              uint32_t *tile) {
     const uint32_t lane = threadIdx.x & 31;
     uint32_t base = 0;
     for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 32) {
         uint32_t first = 0, n = 0;
         if (s0 + lane < b.n_seq) n = seq_rows(b, s0 + lane, &first);
-        const uint32_t nr = n * group;  // below 2^31: the host checks n_tok * group
-        const uint32_t t = nr >= rows_lo && nr < rows_hi ? (nr + rows - 1) / rows : 0;
+        const uint32_t t = (n * group + rows - 1) / rows;  // below 2^31: the host checks n_tok * group
         uint32_t inc = t;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -198,7 +197,6 @@ struct SeqAttnParams {
     uint64_t ld_kv, head_kv;    // elements between rows of k / v, and between a row's kv heads
     uint32_t kv_rows;           // rows of k / v
     uint32_t n_head, n_kv, group, hd, window, n_tiles, splits;
-    uint32_t rows_lo, rows_hi;  // sequences of rows_lo <= n_new * group < rows_hi are this launch's
     float softcap;
 };
 
