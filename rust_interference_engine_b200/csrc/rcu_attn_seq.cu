@@ -6,17 +6,24 @@
 //   o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 //
 // k_attn_seq is the kernel for few query rows per KV head (decode steps, short chunks): it reads
-// every key and value once per 16 query rows and is bound by that reading. A work tile is 16 rows
-// (token, head of the group) of one sequence and KV head; a cluster of CTAs shares it, and every
-// warp of the cluster takes chunks of 16 keys in turn, on its own:
+// every key and value once per work tile (4, 8 or 16 rows: token, head of the group) and is bound by
+// that reading. A cluster of CTAs shares a tile, and every warp of the cluster takes chunks of 16
+// keys in turn, on its own:
 //   * its lane 0 brings a chunk's K and V rows in by tiled TMA (128-byte swizzle) three chunks
 //     ahead, one mbarrier per stage; a chunk lies in one page, so a page may end anywhere;
-//   * S = Q K^T and O += P V with mma.sync m16n8k16 (f32 accumulation): 16 rows fill one fragment;
-//   * running maximum and sum per row in f32. No warp waits for another before its last chunk.
-// Then the warps of a CTA join their states in shared memory and the CTAs of the cluster through
-// distributed shared memory: one launch, and no workspace that two calls or graphs could share.
-// f32 queries: q (scaled by a power of two per row) and p are each split into two f16 parts, so
-// both products carry 22 bits; keys and values are f16 as the cache holds them.
+//   * S^T = K Q^T and O^T += V^T P^T with mma.sync m16n8k16: keys, then values' columns, fill the 16
+//     rows of a fragment and the queries its 8 columns. (With the queries on the 16 rows, four heads
+//     of a group waste three quarters of the products, and mma.sync, at a sixteenth of tcgen05's
+//     rate, becomes the bound: 278 us against 160 us for two f32 sequences of 131,071 keys.)
+//   * running maximum and sum per row in f32; the maximum is raised, and O rescaled, only when a
+//     score passes it by more than 2^kSqLazy, which a vote finds without a reduction over the keys.
+// No warp waits for another before its last chunk. Then the warps of a CTA join their states in
+// shared memory and the CTAs of the cluster through distributed shared memory: one launch, and no
+// workspace that two calls or graphs could share.
+// f32 queries: q (scaled by a power of two per row) and p are each split into two f16 parts that take
+// columns c and c + 4 of one fragment, so both products carry 22 bits; keys and values are f16 as the
+// cache holds them. O is added up outside the MMA, whose own additions do not round to nearest
+// (5.6e-6 off after 131,071 keys).
 #include <cuda.h>
 
 #include <algorithm>
@@ -28,14 +35,14 @@
 
 namespace rcu {
 
-constexpr int kSqRows = 16;     // query rows of a work tile
 constexpr int kSqKeys = 16;     // keys of a chunk
 constexpr int kSqWarps = 4;
 constexpr int kSqStages = 3;
 constexpr int kSqMaxCluster = 16;
-// p is held as 2^kPShift * exp(s - max): in f16 its relative precision then reaches down to
-// 2^-26 of the largest probability; the sum carries the same factor.
-constexpr float kPShift = 12.0f;
+constexpr int kSqMaxRows = 16;
+// p is held as 2^kSqShift * exp(s - m), the row's largest at most 2^(kSqShift + kSqLazy): in f16 its
+// relative precision then reaches down to 2^-21 of exp(0); the sum carries the same factor.
+constexpr float kSqLazy = 8.0f, kSqShift = 7.0f;
 
 template <typename E>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -68,78 +75,33 @@ __device__ __forceinline__ void sq_ldsm_x4_t(uint32_t (&r)[4], uint32_t p) {
 __device__ __forceinline__ uint32_t sq_off(uint32_t r, uint32_t ch, uint32_t rows) {
     return (ch >> 3) * (rows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
 }
+// Transposes an 8 x 8 matrix of 16-bit values held two to a lane.
+__device__ __forceinline__ uint32_t sq_transpose(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 template <int HDP>
 struct SqSmem {
     static constexpr int kTile = kSqKeys * HDP * 2;  // bytes of one chunk's K (or V) rows
     static constexpr int kWarp = kSqStages * 2 * kTile;
-    uint8_t ring[kSqWarps][kWarp];  // at the end: each warp's O, then the CTA's (f32 [16][HDP])
-    float m[kSqWarps][kSqRows], l[kSqWarps][kSqRows];
-    float cm[kSqRows], cl[kSqRows];  // of the CTA
+    static constexpr int kLd = HDP + 4;              // floats between rows of O
+    uint8_t ring[kSqWarps][kWarp];  // at the end: each warp's O, then the CTA's (f32 [rows][kLd])
+    float m[kSqWarps][kSqMaxRows], l[kSqWarps][kSqMaxRows];
+    float cm[kSqMaxRows], cl[kSqMaxRows];  // of the CTA
     uint64_t full[kSqWarps][kSqStages];
+    static_assert(kSqMaxRows * kLd * 4 <= kWarp, "O overlays the ring");
 };
 
-// q as fragments: rows g and g + 8 of the tile, 16 columns a step; f32 rows are scaled by 2^-e
-// (e from the row's largest value) and split in two, and `unscale` is then 2^e.
-template <typename T, typename E, int HDP>
-struct SqFrag {
-    static constexpr bool kSplit = std::is_same<T, float>::value;
-    static constexpr int KS = HDP / 16;
-    uint32_t hi[KS][4], lo[kSplit ? KS : 1][4];
-    float unscale[2];
-
-    __device__ __forceinline__ void load(const SeqAttnParams &p, const SeqSpan &sp, uint32_t kvh, const uint32_t (&row)[2],
-                                         const bool (&live)[2]) {
-        const uint32_t t4 = threadIdx.x & 3;
-        const T *src[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            src[i] = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + row[i] / p.group) * p.ld_q +
-                     (uint64_t)(kvh * p.group + row[i] % p.group) * p.hd;
-        float scale[2] = {1.0f, 1.0f};
-        if constexpr (kSplit) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float mx = 0.0f;
-                for (uint32_t c = 2 * t4; c < p.hd; c += 8)
-                    if (live[i]) mx = fmaxf(mx, fmaxf(fabsf(to_f32(src[i][c])), fabsf(to_f32(src[i][c + 1]))));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                // exponents at which both 2^e and 2^-e are normal numbers
-                const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255), 2), 252) - 127;
-                scale[i] = __uint_as_float((uint32_t)(127 - e) << 23);
-                unscale[i] = __uint_as_float((uint32_t)(127 + e) << 23);
-            }
-        } else {
-            unscale[0] = unscale[1] = 1.0f;
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int i = j & 1;
-                const uint32_t col = 16 * ks + 2 * t4 + (j >= 2 ? 8 : 0);
-                float2 x = make_float2(0.0f, 0.0f);
-                if constexpr (kSplit) {
-                    if (live[i] && col < p.hd) x = *reinterpret_cast<const float2 *>(src[i] + col);
-                    x.x *= scale[i], x.y *= scale[i];
-                    hi[ks][j] = pack2<E>(x.x, x.y);
-                    const float2 h = unpack2<E>(hi[ks][j]);
-                    lo[ks][j] = pack2<E>(x.x - h.x, x.y - h.y);
-                } else {
-                    hi[ks][j] = live[i] && col < p.hd ? *reinterpret_cast<const uint32_t *>(src[i] + col) : 0u;
-                }
-            }
-        }
-    }
-};
-
-template <typename T, typename E, int HDP>
+template <typename T, typename E, int HDP, int NT>
 __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constant__ CUtensorMap mk,
                                                             const __grid_constant__ CUtensorMap mv,
                                                             const __grid_constant__ SeqAttnParams p) {
     using S = SqSmem<HDP>;
     constexpr bool kSplit = std::is_same<T, float>::value;
-    constexpr int KS = HDP / 16, NO = HDP / 8;
+    constexpr int KS = HDP / 16;
+    constexpr int kPer = kSplit ? 4 : 8, kRows = kPer * NT;  // rows of a fragment, of the tile
     extern __shared__ uint8_t sq_raw[];
     S &sm = *reinterpret_cast<S *>((reinterpret_cast<uintptr_t>(sq_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -149,30 +111,20 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
     pdl_trigger();
     SeqSpan sp;
     uint32_t tile;
-    if (!seq_find_tile(p.b, p.group, kSqRows, ti, &sp, &tile)) return;  // the same for the whole cluster
+    if (!seq_find_tile(p.b, p.group, kRows, ti, &sp, &tile)) return;  // the same for the whole cluster
     if (lane == 0) {
         for (int s = 0; s < kSqStages; s++) mbar_init(&sm.full[warp][s], 1);
         fence_mbar_init();
     }
     __syncwarp();
-    const uint32_t row0 = tile * kSqRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kSqRows);
-    // attended positions [lo, hi] of this thread's two rows (none: hi = -1) and of the whole tile
-    uint32_t row[2];
-    bool live[2];
-    int64_t lo[2], hi[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        live[i] = g + 8 * i < n_rows;
-        row[i] = row0 + min(g + 8 * i, n_rows - 1);
-        hi[i] = live[i] ? sp.pos(row[i] / p.group) : -1;
-        lo[i] = p.window > 0 && hi[i] + 1 > (int64_t)p.window ? hi[i] + 1 - p.window : 0;
-    }
-    const int64_t p_first = sp.pos(row0 / p.group), k_hi = sp.pos((row0 + n_rows - 1) / p.group);
-    const int64_t k_lo = p.window > 0 && p_first + 1 > (int64_t)p.window ? p_first + 1 - p.window : 0;
+    const uint32_t row0 = tile * kRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kRows);
+    // the tile's attended positions k_lo .. k_hi; positions stay below 2^31
+    const int32_t p_first = (int32_t)sp.pos(row0 / p.group), k_hi = (int32_t)sp.pos((row0 + n_rows - 1) / p.group);
+    const int32_t k_lo = p.window > 0 ? max(p_first - (int32_t)p.window + 1, 0) : 0;
     const uint32_t c_lo = (uint32_t)(k_lo / kSqKeys), c_all = k_hi >= 0 ? (uint32_t)(k_hi / kSqKeys) + 1 : 0;
     const uint32_t n_chunks = c_all > c_lo ? c_all - c_lo : 0;
     // keys that every live row attends: chunks inside need no mask
-    const int64_t all_lo = p.window > 0 && k_hi + 1 > (int64_t)p.window ? k_hi + 1 - p.window : 0, all_hi = p_first;
+    const int32_t all_lo = p.window > 0 ? max(k_hi - (int32_t)p.window + 1, 0) : 0, all_hi = p_first;
 
     // this warp's chunks: w0, w0 + stride, ... of the tile's n_chunks
     const uint32_t stride = p.splits * kSqWarps, w0 = rank * kSqWarps + warp;
@@ -183,11 +135,10 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
         const uint32_t i = i0 + lane;
         rows_ahead = i < mine ? seq_kv_row(p.b, sp, p.n_kv, kvh, (c_lo + w0 + i * stride) * kSqKeys) : 0;
     };
-    auto issue = [&](uint32_t i) {  // whole warp; brings chunk i into stage i % kSqStages
+    auto issue = [&](uint32_t i, uint32_t st) {  // whole warp; brings chunk i into stage st = i % kSqStages
         if ((i & 31) == 0) fetch_rows(i);
         const uint32_t r = __shfl_sync(0xffffffffu, rows_ahead, i & 31);
         if (lane == 0) {
-            const uint32_t st = i % kSqStages;
             uint8_t *kd = ring + st * 2 * S::kTile, *vd = kd + S::kTile;
             // a page number out of range reads as zeros: rows behind the tensor's end
             const int y = (int)min(r, p.kv_rows), h = p.b.pages ? 0 : (int)kvh;
@@ -199,135 +150,204 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
             }
         }
     };
-    const uint32_t pre = min(mine, (uint32_t)kSqStages);
-    for (uint32_t i = 0; i < pre; i++) issue(i);
+    for (uint32_t i = 0; i < min(mine, (uint32_t)kSqStages); i++) issue(i, i);
 
-    SqFrag<T, E, HDP> q;
-    q.load(p, sp, kvh, row, live);
-    const float sc[2] = {q.unscale[0] * kLog2e, q.unscale[1] * kLog2e};
-    float o[NO][4];
+    // q as B fragments: column g of fragment n (f32: row 4 n + g % 4, its high part in columns 0-3, the
+    // rest in 4-7, the row scaled by 2^-e, e from its largest value)
+    uint32_t q[NT][KS][2];
+    float unscale[NT][2];  // 2^e of this thread's score rows
 #pragma unroll
-    for (int n = 0; n < NO; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // m in units of log2
+    for (int n = 0; n < NT; n++) {
+        const uint32_t r = kPer * n + g % kPer, rr = row0 + min(r, n_rows - 1);
+        const bool live = r < n_rows;
+        const T *src = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + rr / p.group) * p.ld_q +
+                       (uint64_t)(kvh * p.group + rr % p.group) * p.hd;
+        if constexpr (kSplit) {
+            float2 x[KS][2];
+            float mx = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t col = 16 * ks + 8 * j + 2 * t4;
+                    x[ks][j] = live && col < p.hd ? *reinterpret_cast<const float2 *>(src + col) : make_float2(0.0f, 0.0f);
+                    mx = fmaxf(mx, fmaxf(fabsf(x[ks][j].x), fabsf(x[ks][j].y)));
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // exponents at which both 2^e and 2^-e are normal numbers
+            const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255), 2), 252) - 127;
+            const float scale = __uint_as_float((uint32_t)(127 - e) << 23), un = __uint_as_float((uint32_t)(127 + e) << 23);
+            unscale[n][0] = __shfl_sync(0xffffffffu, un, 4 * (2 * (t4 & 1)));
+            unscale[n][1] = __shfl_sync(0xffffffffu, un, 4 * (2 * (t4 & 1) + 1));
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float a = x[ks][j].x * scale, b = x[ks][j].y * scale;
+                    const uint32_t h = pack2<E>(a, b);
+                    const float2 f = unpack2<E>(h);
+                    q[n][ks][j] = g < 4 ? h : pack2<E>(a - f.x, b - f.y);
+                }
+        } else {
+            unscale[n][0] = unscale[n][1] = 1.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t col = 16 * ks + 8 * j + 2 * t4;
+                    q[n][ks][j] = live && col < p.hd ? *reinterpret_cast<const uint32_t *>(src + col) : 0u;
+                }
+        }
+    }
+    float sc[NT][2];  // scores times sc are in units of log2
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) sc[n][i] = p.softcap > 0.0f ? 1.0f : unscale[n][i] * kLog2e;
+    // this thread's scores: keys g and g + 8 of a chunk, rows srow[n][0..1] of the tile, which attend
+    // positions slo .. shi
+    int32_t slo[NT][2], shi[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint32_t r = kPer * n + (2 * t4 + i) % kPer;
+            shi[n][i] = r < n_rows ? (int32_t)sp.pos((row0 + r) / p.group) : -1;
+            slo[n][i] = p.window > 0 ? max(shi[n][i] - (int32_t)p.window + 1, 0) : 0;
+        }
+    float o[NT][KS][4];  // O^T: columns 16 ks + g (+ 8) of rows as the scores' (f32: high parts, the rest)
+    float m[NT][2], l[NT][2];  // m in units of log2
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) o[n][ks][0] = o[n][ks][1] = o[n][ks][2] = o[n][ks][3] = 0.0f;
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+    }
 
     bool ok = true;
+    uint32_t st = 0, parity = 0;
+    const uint32_t mi = lane >> 3, l7 = lane & 7;
     for (uint32_t i = 0; i < mine; i++) {
-        const uint32_t st = i % kSqStages;
-        ok = mbar_wait_bounded(&sm.full[warp][st], (i / kSqStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
+        ok = mbar_wait_spin(&sm.full[warp][st], parity, p.b.err, ERR_TIMEOUT_FULL);
         if (!ok) {  // the result is void; the copies still in flight must land before the CTA ends
             for (uint32_t j = i + 1; j < min(mine, i + kSqStages); j++)
-                mbar_wait_bounded(&sm.full[warp][j % kSqStages], (j / kSqStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
+                mbar_wait_spin(&sm.full[warp][j % kSqStages], (j / kSqStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
             break;
         }
+        uint8_t *vrows = ring + st * 2 * S::kTile + S::kTile;
         const uint32_t kb = smem_u32(ring + st * 2 * S::kTile), vb = kb + S::kTile;
-        const int64_t c0 = (int64_t)(c_lo + w0 + i * stride) * kSqKeys;
-        float s[2][4] = {};
-        const int mi = lane >> 3;
+        const int32_t c0 = (int32_t)(c_lo + w0 + i * stride) * kSqKeys;
+        const bool part = c0 < all_lo || c0 + kSqKeys - 1 > all_hi;
+        if (c0 + kSqKeys - 1 > k_hi) {  // rows behind the last key hold anything: 0 * v must stay 0
+            for (uint32_t r = (uint32_t)(k_hi - c0 + 1); r < kSqKeys; r++)
+                for (uint32_t c = lane; c < HDP / 8; c += 32)
+                    *reinterpret_cast<uint4 *>(vrows + sq_off(r, c, kSqKeys)) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
+            __syncwarp();
+        }
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             uint32_t r[4];
-            sq_ldsm_x4(r, kb + sq_off(8 * (mi >> 1) + (lane & 7), 2 * ks + (mi & 1), kSqKeys));
-            mma_16816<E>(s[0], q.hi[ks], r[0], r[1]);
-            mma_16816<E>(s[1], q.hi[ks], r[2], r[3]);
-            if constexpr (kSplit) {
-                mma_16816<E>(s[0], q.lo[ks], r[0], r[1]);
-                mma_16816<E>(s[1], q.lo[ks], r[2], r[3]);
+            sq_ldsm_x4(r, kb + sq_off(8 * (mi & 1) + l7, 2 * ks + (mi >> 1), kSqKeys));
+#pragma unroll
+            for (int n = 0; n < NT; n++) mma_16816<E>(s[n], r, q[n][ks][0], q[n][ks][1]);
+        }
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {  // key g + 8 (j >> 1), row j & 1
+                float v = s[n][j];
+                if constexpr (kSplit) v += __shfl_xor_sync(0xffffffffu, v, 2);
+                if (p.softcap > 0.0f) v = p.softcap * kLog2e * tanhf(v * unscale[n][j & 1] / p.softcap);
+                if (part) {
+                    const int32_t key = c0 + (int32_t)g + 8 * (j >> 1);
+                    if (key > shi[n][j & 1] || key < slo[n][j & 1]) v = -INFINITY;
+                }
+                s[n][j] = v;
+                v *= sc[n][j & 1];
+                grow |= v > m[n][j & 1] + kSqLazy || (m[n][j & 1] == -INFINITY && v > -INFINITY);
             }
-        }
-        // s in units of log2, masked where the chunk is not attended by every row
-        if (p.softcap > 0.0f) {
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[n][j] = p.softcap * kLog2e * tanhf(s[n][j] * q.unscale[j >> 1] / p.softcap);
-        }
-        const bool part = c0 < all_lo || c0 + kSqKeys - 1 > all_hi;
-        float mx[2] = {-INFINITY, -INFINITY};
-        if (part) {
+                for (int k = 0; k < 2; k++) {
+                    float mx = fmaxf(fmaxf(s[n][k], s[n][2 + k]) * sc[n][k], m[n][k]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float a = mx == m[n][k] ? 1.0f : ex2(m[n][k] - mx);
+                    m[n][k] = mx;
+                    l[n][k] *= a;
 #pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int64_t kp = c0 + 8 * n + 2 * t4 + (j & 1);
-                    if (kp > hi[j >> 1] || kp < lo[j >> 1]) s[n][j] = -INFINITY;
+                    for (int ks = 0; ks < KS; ks++) o[n][ks][k] *= a, o[n][ks][2 + k] *= a;
                 }
         }
-        const float cs[2] = {p.softcap > 0.0f ? 1.0f : sc[0], p.softcap > 0.0f ? 1.0f : sc[1]};
+        uint32_t b[NT][2];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < NT; n++) {
+            float e[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) mx[j >> 1] = fmaxf(mx[j >> 1], s[n][j]);
-        bool grew = false;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
-            mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
-            mx[k] *= cs[k];  // cs > 0
-            grew |= mx[k] > m[k];
-        }
-        if (__any_sync(0xffffffffu, grew)) {
+            for (int j = 0; j < 4; j++) {
+                e[j] = ex2(fmaf(s[n][j], sc[n][j & 1], kSqShift - (m[n][j & 1] == -INFINITY ? 0.0f : m[n][j & 1])));
+                l[n][j & 1] += e[j];
+            }
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                const float mn = fmaxf(m[k], mx[k]);
-                const float a = mn == -INFINITY ? 1.0f : ex2(m[k] - mn);
-                m[k] = mn;
-                l[k] *= a;
-#pragma unroll
-                for (int n = 0; n < NO; n++) o[n][2 * k] *= a, o[n][2 * k + 1] *= a;
-            }
-        }
-        float pr[2][4];
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const float off = (m[k] == -INFINITY ? 0.0f : m[k]) - kPShift;
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float e = ex2(fmaf(s[n][2 * k + j], cs[k], -off));
-                    pr[n][2 * k + j] = e;
-                    l[k] += e;
+                uint32_t u = pack2<E>(e[2 * k], e[2 * k + 1]);
+                if constexpr (kSplit) {
+                    const float2 f = unpack2<E>(u);
+                    if (t4 >= 2) u = pack2<E>(e[2 * k] - f.x, e[2 * k + 1] - f.y);
                 }
-        }
-        uint32_t ah[4], al[4];
-        const float pv[4][2] = {{pr[0][0], pr[0][1]}, {pr[0][2], pr[0][3]}, {pr[1][0], pr[1][1]}, {pr[1][2], pr[1][3]}};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            ah[j] = pack2<E>(pv[j][0], pv[j][1]);
-            if constexpr (kSplit) {
-                const float2 h = unpack2<E>(ah[j]);
-                al[j] = pack2<E>(pv[j][0] - h.x, pv[j][1] - h.y);
+                b[n][k] = sq_transpose(u);
             }
         }
 #pragma unroll
-        for (int nd = 0; nd < HDP / 16; nd++) {
+        for (int ks = 0; ks < KS; ks++) {
             uint32_t r[4];
-            sq_ldsm_x4_t(r, vb + sq_off(8 * (mi & 1) + (lane & 7), 2 * nd + (mi >> 1), kSqKeys));
-            mma_16816<E>(o[2 * nd], ah, r[0], r[1]);
-            mma_16816<E>(o[2 * nd + 1], ah, r[2], r[3]);
-            if constexpr (kSplit) {
-                mma_16816<E>(o[2 * nd], al, r[0], r[1]);
-                mma_16816<E>(o[2 * nd + 1], al, r[2], r[3]);
+            sq_ldsm_x4_t(r, vb + sq_off(8 * (mi >> 1) + l7, 2 * ks + (mi & 1), kSqKeys));
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if constexpr (kSplit) {
+                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_16816<E>(d, r, b[n][0], b[n][1]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[n][ks][j] += d[j];
+                } else {
+                    mma_16816<E>(o[n][ks], r, b[n][0], b[n][1]);
+                }
             }
         }
         __syncwarp();  // every lane has read the stage
-        if (i + kSqStages < mine) issue(i + kSqStages);
+        if (i + kSqStages < mine) issue(i + kSqStages, st);
+        if (++st == kSqStages) st = 0, parity ^= 1;
     }
     // ---- join: warps of the CTA, then CTAs of the cluster -----------------------------------------
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
-        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
-        if (t4 == 0) sm.m[warp][g + 8 * k] = m[k], sm.l[warp][g + 8 * k] = l[k];
-    }
     // this warp's ring is free (all its copies were waited for, or its wait ran out and the result is void)
     float *ow = reinterpret_cast<float *>(ring);
-    if (ok) {
 #pragma unroll
-        for (int n = 0; n < NO; n++)
+    for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int k = 0; k < 2; k++)
-                *reinterpret_cast<float2 *>(ow + (g + 8 * k) * HDP + 8 * n + 2 * t4) = make_float2(o[n][2 * k], o[n][2 * k + 1]);
+        for (int k = 0; k < 2; k++) {
+            l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], 4);
+            l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], 8);
+            l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], 16);
+            if (g == 0 && 2 * t4 < kPer) sm.m[warp][kPer * n + 2 * t4 + k] = m[n][k], sm.l[warp][kPer * n + 2 * t4 + k] = l[n][k];
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float v = o[n][ks][j];
+                if constexpr (kSplit) v += __shfl_xor_sync(0xffffffffu, v, 2);
+                if (2 * t4 < kPer && ok) ow[(kPer * n + 2 * t4 + (j & 1)) * S::kLd + 16 * ks + g + 8 * (j >> 1)] = v;
+            }
     }
     __syncthreads();
     float *oc = reinterpret_cast<float *>(sm.ring[0]);
@@ -346,8 +366,8 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
             float acc = 0.0f;
 #pragma unroll
             for (int w = 0; w < kSqWarps; w++)
-                if (a[w] != 0.0f) acc += a[w] * oc[w * kOw + r * HDP + d];
-            oc[r * HDP + d] = acc;
+                if (a[w] != 0.0f) acc += a[w] * oc[w * kOw + r * S::kLd + d];
+            oc[r * S::kLd + d] = acc;
         }
         if (lane == 0) sm.cm[r] = M, sm.cl[r] = L;
     }
@@ -359,9 +379,9 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
         float acc[HDP / 32] = {};
         if (p.splits == 1) {
             L = sm.cl[r];
-            for (int i = 0; i < HDP / 32; i++) acc[i] = oc[r * HDP + lane + 32 * i];
+            for (int i = 0; i < HDP / 32; i++) acc[i] = oc[r * S::kLd + lane + 32 * i];
         } else {
-            const uint32_t am = smem_u32(&sm.cm[r]), al2 = smem_u32(&sm.cl[r]), ao = smem_u32(oc + r * HDP + lane);
+            const uint32_t am = smem_u32(&sm.cm[r]), al2 = smem_u32(&sm.cl[r]), ao = smem_u32(oc + r * S::kLd + lane);
             const float mc = lane < p.splits ? ld_cluster_f32(cluster_addr(am, lane)) : -INFINITY;
             const float lc = lane < p.splits ? ld_cluster_f32(cluster_addr(al2, lane)) : 0.0f;
             M = mc;
@@ -398,9 +418,10 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-template <typename T, typename E, int HDP>
+template <typename T, typename E, int HDP, int NT>
 static int launch_few(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv, SeqAttnParams p, uint64_t max_len) {
     const size_t smem = sizeof(SqSmem<HDP>) + 1024;
+    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, (std::is_same<T, float>::value ? 4 : 8) * NT);
     // CTAs per tile: up to two for each SM in all, and at least 128 keys each
     const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + 16) : max_len;
     const uint32_t most = HDP == 256 ? 8 : kSqMaxCluster;  // 197 KB of shared memory each: eight SMs of a GPC are sure to be there
@@ -408,23 +429,29 @@ static int launch_few(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv
     while (cs < most && items * cs * 2 <= 2ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 128) cs *= 2;
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
-    return launch_cluster_k(ctx, k_attn_seq<T, E, HDP>, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, mk, mv, p);
+    return launch_cluster_k(ctx, k_attn_seq<T, E, HDP, NT>, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, mk, mv, p);
 }
 
+// One fragment of rows where they fill no more (a group's heads for single tokens), else two.
 template <typename T, typename E>
-static int launch_few_hd(rcu_ctx *ctx, SeqAttnParams p, const SeqKvDesc &kv, uint64_t max_len) {
+static int launch_few_hd(rcu_ctx *ctx, const SeqAttnParams &p, const SeqKvDesc &kv, uint64_t max_len, uint64_t most) {
     CUtensorMap mk, mv;
     if (int st = seq_kv_maps(ctx, p, kv, kSqKeys, &mk, &mv)) return st;
-    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kSqRows);
-    if (p.hd <= 64) return launch_few<T, E, 64>(ctx, mk, mv, p, max_len);
-    if (p.hd <= 128) return launch_few<T, E, 128>(ctx, mk, mv, p, max_len);
-    return launch_few<T, E, 256>(ctx, mk, mv, p, max_len);
+    if (most <= (std::is_same<T, float>::value ? 4u : 8u)) {
+        if (p.hd <= 64) return launch_few<T, E, 64, 1>(ctx, mk, mv, p, max_len);
+        if (p.hd <= 128) return launch_few<T, E, 128, 1>(ctx, mk, mv, p, max_len);
+        return launch_few<T, E, 256, 1>(ctx, mk, mv, p, max_len);
+    }
+    if (p.hd <= 64) return launch_few<T, E, 64, 2>(ctx, mk, mv, p, max_len);
+    if (p.hd <= 128) return launch_few<T, E, 128, 2>(ctx, mk, mv, p, max_len);
+    return launch_few<T, E, 256, 2>(ctx, mk, mv, p, max_len);
 }
 
-static int launch_attention_few(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len) {
-    if (q_type == T_F32) return launch_few_hd<float, __half>(ctx, p, kv, max_len);
-    if (q_type == T_F16) return launch_few_hd<__half, __half>(ctx, p, kv, max_len);
-    return launch_few_hd<__nv_bfloat16, __nv_bfloat16>(ctx, p, kv, max_len);
+static int launch_attention_few(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,
+                                uint64_t most) {
+    if (q_type == T_F32) return launch_few_hd<float, __half>(ctx, p, kv, max_len, most);
+    if (q_type == T_F16) return launch_few_hd<__half, __half>(ctx, p, kv, max_len, most);
+    return launch_few_hd<__nv_bfloat16, __nv_bfloat16>(ctx, p, kv, max_len, most);
 }
 
 int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,
@@ -434,9 +461,9 @@ int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const
     // takes the whole batch: in a mixed one the single tokens ride along with the chunks (two chunks
     // of 333 tokens beside 14 single ones: 64 us for the chunks alone and 62 us for the single
     // tokens in a launch of their own).
-    const uint64_t most = std::min<uint64_t>(max_new ? max_new : p.b.n_tok, p.b.n_tok) * p.group;
-    if (!attention_tile_ok(p.hd) || most < kTileMinRows || (!max_new && p.b.n_tok <= p.b.n_seq))
-        return launch_attention_few(ctx, p, q_type, kv, max_len);
+    const uint64_t new_max = max_new ? max_new : p.b.n_tok <= p.b.n_seq ? 1 : p.b.n_tok;
+    const uint64_t most = std::min<uint64_t>(new_max, p.b.n_tok) * p.group;
+    if (!attention_tile_ok(p.hd) || most < kTileMinRows) return launch_attention_few(ctx, p, q_type, kv, max_len, most);
     return launch_attention_tile(ctx, p, q_type, kv, max_len);
 }
 

@@ -330,6 +330,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         constexpr uint32_t kIdO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(HDP >> 3) << 17) | (8u << 24);
         auto uni = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
         const int32_t n_blk = uni(j1 - j0), b0 = uni(jb[0] - j0), e0 = uni(je[0] - j0), b1 = uni(jb[1] - j0), e1 = uni(je[1] - j0);
+        // keys from this CTA's first block to the last one that a row attends
+        const int32_t n_keys = uni((int32_t)(sp.pos((row0 + n_rows - 1) / p.group) + 1 - (int64_t)j0 * kTlBlk));
         const uint32_t tm = uni((int32_t)tmem);
         const uint64_t dq = sw128_desc(sm.data), dk = sw128_desc(ring), dv = sw128_desc_mn(ring, kTlBlk * 128);
         const bool elected = elect_one();
@@ -343,7 +345,17 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         uint32_t sk = 0, pk = 0, sv = 1, pv = 0;  // ring stage and parity of K(j), V(j - 1)
         for (int32_t j = 0; j <= n_blk && ok; j++) {
             const bool last = j == n_blk;
-            if (j > 0) wait(&sm.full[sv], pv);
+            if (j > 0) {
+                wait(&sm.full[sv], pv);
+                if (j * kTlBlk > n_keys) {  // rows behind the last key hold anything: 0 * v must stay 0
+                    uint8_t *v = ring + sv * C::kStage;
+                    for (uint32_t i = (uint32_t)(n_keys - (j - 1) * kTlBlk) * 8 + lane; i < kTlBlk * 8; i += 32)
+#pragma unroll
+                        for (int c = 0; c < kChunks; c++) *reinterpret_cast<uint4 *>(v + c * (kTlBlk * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+            }
             if (!last) wait(&sm.full[sk], pk);
 #pragma unroll
             for (int t = 0; t < 2; t++) {
