@@ -9,7 +9,7 @@
 // every key and value once per work tile (4, 8 or 16 rows: token, head of the group) and is bound by
 // that reading. A cluster of CTAs shares a tile, and every warp of the cluster takes chunks of 16
 // keys in turn, on its own:
-//   * its lane 0 brings a chunk's K and V rows in by tiled TMA (128-byte swizzle) three chunks
+//   * its lane 0 brings a chunk's K and V rows in by tiled TMA (128-byte swizzle) two chunks
 //     ahead, one mbarrier per stage; a chunk lies in one page, so a page may end anywhere;
 //   * S^T = K Q^T and O^T += V^T P^T with mma.sync m16n8k16: keys, then values' columns, fill the 16
 //     rows of a fragment and the queries its 8 columns. (With the queries on the 16 rows, four heads
@@ -37,7 +37,7 @@ namespace rcu {
 
 constexpr int kSqKeys = 16;     // keys of a chunk
 constexpr int kSqWarps = 4;
-constexpr int kSqStages = 3;
+constexpr int kSqStages = 2;  // three CTAs to an SM; with three stages two, of which clusters of 16 leave SMs idle (199 against 159 us)
 constexpr int kSqMaxCluster = 16;
 constexpr int kSqMaxRows = 16;
 // p is held as 2^kSqShift * exp(s - m), the row's largest at most 2^(kSqShift + kSqLazy): in f16 its
@@ -422,11 +422,11 @@ template <typename T, typename E, int HDP, int NT>
 static int launch_few(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv, SeqAttnParams p, uint64_t max_len) {
     const size_t smem = sizeof(SqSmem<HDP>) + 1024;
     p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, (std::is_same<T, float>::value ? 4 : 8) * NT);
-    // CTAs per tile: up to two for each SM in all, and at least 128 keys each
+    // CTAs per tile: up to three for each SM in all, and at least 128 keys each
     const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + 16) : max_len;
-    const uint32_t most = HDP == 256 ? 8 : kSqMaxCluster;  // 197 KB of shared memory each: eight SMs of a GPC are sure to be there
+    const uint32_t most = HDP == 256 ? 8 : kSqMaxCluster;  // one CTA to an SM: eight SMs of a GPC are sure to be there
     uint32_t cs = 1;
-    while (cs < most && items * cs * 2 <= 2ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 128) cs *= 2;
+    while (cs < most && items * cs * 2 <= 3ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 128) cs *= 2;
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
     return launch_cluster_k(ctx, k_attn_seq<T, E, HDP, NT>, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, mk, mv, p);

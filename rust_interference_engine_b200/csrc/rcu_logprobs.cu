@@ -5,13 +5,15 @@
 //   log p(i) = (x_i - m) - ln z          entropy = ln z - (sum exp(x - m) (x - m)) / z
 // and the top_k largest, ties to the lowest index (a NaN counts as the largest value, -0 as 0).
 //
-// Reading the logits is the bound. A cluster of `splits` CTAs shares a row, each thread keeps a
-// running (m, z, sum) over the values it reads, 16 a step. The alternatives need no second pass: a
-// value is a 64-bit key (ordered value, ~index), and after the first step the k-th largest of the
-// threads' own maxima is a bound below which nothing can be among the k largest of the row; a later
-// value reaches the candidate list in shared memory only above it. When that list could run over,
-// the same bound is taken again from the list itself. The list's ranks, by counting larger keys,
-// are the order of the answer.
+// Reading the logits is the bound. A cluster of `splits` CTAs shares a row; each thread keeps a
+// running (m, z, sum) over the values it reads, 16 a step, the next step's loads on their way
+// meanwhile. The alternatives need no second pass: a value is a 64-bit key (ordered value, ~index),
+// and the k-th largest of some threads' own maxima is a bound below which nothing can be among the k
+// largest of the row. A value reaches the candidate list in shared memory only above the bound, which
+// is taken from the first step's maxima and again from the list after 2, 4, 8, ... steps; no other
+// step has a barrier. Should the list run over all the same (logits that rise along the row), the
+// CTA reads its part again with a check after every step. The candidates' ranks, by counting larger
+// keys, are the order of the answer.
 #include <cstdint>
 #include <type_traits>
 
@@ -20,19 +22,19 @@
 
 namespace rcu {
 
-constexpr int kLpThreads = 256;
 constexpr int kLpPer = 16;                       // values a thread reads per step
-constexpr int kLpStep = kLpThreads * kLpPer;
 constexpr int kLpMaxTop = 128;
 constexpr int kLpMaxSplits = 16;
-constexpr int kLpKeep = 1024;                    // candidates kept over a step at most
-constexpr int kLpCap = kLpKeep + kLpStep;
+constexpr int kLpCap = 2048;                     // candidates
+constexpr int kLpBound = 256;                    // threads whose maxima give a bound
+// A checked step adds at most kLpCap / 2 candidates to at most as many that are kept.
+constexpr int kLpKeep = kLpCap / 2;
 
 struct LpSmem {
     uint64_t cand[kLpCap];
-    uint64_t tmax[kLpThreads];
+    uint64_t tmax[kLpBound];
     uint64_t top[kLpMaxTop];      // this CTA's largest keys in order
-    float rm[8], rz[8], rw[8];
+    float rm[32], rz[32], rw[32];
     float cm, cz, cw;             // of the CTA
     uint32_t n;
     uint64_t bound;
@@ -79,27 +81,34 @@ struct LpSum {
     }
 };
 
-// k-th largest of the threads' keys `mine` (0: no key): a lower bound of the k-th largest of all
-// keys that the threads' own maxima stand for; 0 when fewer than k threads have a key.
+// k-th largest of the keys `mine` of threads 0 .. kLpBound - 1 (0: no key): a lower bound of the
+// k-th largest of all keys that these threads' own maxima stand for; 0 when fewer than k have one.
 __device__ __forceinline__ uint64_t lp_bound(LpSmem &sm, uint64_t mine, uint32_t k) {
-    sm.tmax[threadIdx.x] = mine;
+    if (threadIdx.x < kLpBound) sm.tmax[threadIdx.x] = mine;
     if (threadIdx.x == 0) sm.bound = 0;
     __syncthreads();
-    uint32_t above = 0;
+    if (threadIdx.x < kLpBound && mine != 0) {
+        uint32_t above = 0;
+        const ulonglong2 *t = reinterpret_cast<const ulonglong2 *>(sm.tmax);
 #pragma unroll 8
-    for (int i = 0; i < kLpThreads; i++) above += sm.tmax[i] > mine;
-    if (mine != 0 && above == k - 1) sm.bound = mine;  // keys differ: one thread at most
+        for (int i = 0; i < kLpBound / 2; i++) {
+            const ulonglong2 x = t[i];
+            above += (x.x > mine) + (x.y > mine);
+        }
+        if (above == k - 1) sm.bound = mine;  // keys differ: one thread at most
+    }
     __syncthreads();
     return sm.bound;
 }
-// Raises the bound from the candidate list itself and drops what lies below it.
+// Raises the bound from the candidate list itself and drops what lies below it: at most
+// k * ceil(n / kLpBound) <= n / 2 + 128 candidates stay. The whole CTA.
 __device__ __noinline__ uint64_t lp_compact(LpSmem &sm, uint32_t n, uint32_t k) {
-    constexpr int kMost = (kLpCap + kLpThreads - 1) / kLpThreads;
+    constexpr int kMost = kLpCap / kLpBound;
     uint64_t own[kMost], mx = 0;
 #pragma unroll
     for (int i = 0; i < kMost; i++) {
-        const uint32_t j = threadIdx.x + i * kLpThreads;
-        own[i] = j < n ? sm.cand[j] : 0;
+        const uint32_t j = threadIdx.x + i * kLpBound;
+        own[i] = threadIdx.x < kLpBound && j < n ? sm.cand[j] : 0;
         mx = own[i] > mx ? own[i] : mx;
     }
     const uint64_t bound = lp_bound(sm, mx, k);
@@ -112,10 +121,71 @@ __device__ __noinline__ uint64_t lp_compact(LpSmem &sm, uint32_t n, uint32_t k) 
     return bound;
 }
 
+// A row's part as a CTA reads it: 16-byte pieces v0 .. v1 - 1, counted from the boundary at or below
+// the row's start; a row may start and end inside one.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, uint32_t splits) {
-    constexpr int VE = 16 / sizeof(T);      // values of a 16-byte load
-    constexpr int NV = kLpPer / VE;         // loads a step
+struct LpPart {
+    static constexpr int VE = 16 / sizeof(T);
+    const T *x;
+    uint32_t off, vocab, v0, v1;
+    __device__ __forceinline__ uint32_t index(uint32_t v, int i) const { return v * VE + i - off; }  // of value i of piece v
+    __device__ __forceinline__ bool inside(uint32_t v) const { return v < v1 && v * VE >= off && v * VE + VE - off <= vocab; }
+    __device__ __forceinline__ bool valid(uint32_t v, int i) const { return v < v1 && v * VE + i >= off && v * VE + i - off < vocab; }
+    // piece v (outside values: -inf)
+    __device__ __forceinline__ uint4 load(uint32_t v) const {
+        if (inside(v)) return __ldcs(reinterpret_cast<const uint4 *>(x - off) + v);
+        alignas(16) T t[VE];
+#pragma unroll
+        for (int i = 0; i < VE; i++) t[i] = valid(v, i) ? x[index(v, i)] : from_f32<T>(-INFINITY);
+        return *reinterpret_cast<const uint4 *>(t);
+    }
+    static __device__ __forceinline__ void values(const uint4 &u, float *f) {
+        if constexpr (sizeof(T) == 4) {
+            f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+        } else {
+            const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y), c = unpack2<T>(u.z), d = unpack2<T>(u.w);
+            f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
+        }
+    }
+};
+
+// The candidates once more, for a list that ran over: one piece a thread and step (at most kLpKeep
+// values), the list cut down after each.
+template <typename T, int THREADS>
+__device__ __noinline__ void lp_checked(LpSmem &sm, const LpPart<T> &part, uint32_t k) {
+    constexpr int VE = LpPart<T>::VE, kTake = kLpKeep / VE < THREADS ? kLpKeep / VE : THREADS;
+    uint64_t bound = 0;
+    __syncthreads();
+    if (threadIdx.x == 0) sm.n = 0;
+    __syncthreads();
+    for (uint32_t s = part.v0; s < part.v1; s += kTake) {
+        const uint32_t v = s + threadIdx.x;
+        if (threadIdx.x < kTake && v < part.v1) {
+            float f[VE];
+            LpPart<T>::values(part.load(v), f);
+#pragma unroll
+            for (int i = 0; i < VE; i++)
+                if (part.valid(v, i)) {
+                    const uint64_t key = lp_key(f[i], part.index(v, i));
+                    if (key >= bound) sm.cand[atomicAdd(&sm.n, 1u)] = key;
+                }
+        }
+        __syncthreads();
+        uint32_t n = sm.n;
+        __syncthreads();
+        while (n > (uint32_t)kLpKeep) {
+            bound = lp_compact(sm, n, k);
+            n = sm.n;
+            __syncthreads();
+        }
+    }
+}
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_logprobs(const LogprobParams p, uint32_t splits) {
+    using Part = LpPart<T>;
+    constexpr int VE = Part::VE, NV = kLpPer / VE;  // values of a 16-byte load, loads a step
+    constexpr uint32_t kStep = THREADS * NV;
     extern __shared__ __align__(16) uint8_t lp_raw[];
     LpSmem &sm = *reinterpret_cast<LpSmem *>(lp_raw);
     const uint32_t rank = splits > 1 ? cluster_ctarank() : 0, r = blockIdx.x / splits, k = p.top_k;
@@ -124,82 +194,80 @@ __global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, 
     __syncthreads();
     pdl_wait();
     pdl_trigger();
-    const T *x = reinterpret_cast<const T *>(p.logits) + (uint64_t)r * p.ld;
-    // 16-byte pieces of the row, counted from the boundary at or below its start
-    const uint32_t off = (uint32_t)(((uintptr_t)x & 15) / sizeof(T));
-    const T *base = x - off;
-    const uint32_t n_vec = (off + p.vocab + VE - 1) / VE, per = (n_vec + splits - 1) / splits;
-    const uint32_t v0 = min(rank * per, n_vec), v1 = min(v0 + per, n_vec);
+    Part part;
+    part.x = reinterpret_cast<const T *>(p.logits) + (uint64_t)r * p.ld;
+    part.off = (uint32_t)(((uintptr_t)part.x & 15) / sizeof(T));
+    part.vocab = p.vocab;
+    const uint32_t n_vec = (part.off + p.vocab + VE - 1) / VE, per = (n_vec + splits - 1) / splits;
+    part.v0 = min(rank * per, n_vec), part.v1 = min(part.v0 + per, n_vec);
+    const T *x = part.x;
 
     LpSum a;
     uint64_t bound = 0;
     float boundf = -INFINITY;
-    for (uint32_t s = v0; s < v1; s += kLpThreads * NV) {
+    uint32_t done = 0;  // steps
+    uint4 next[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) next[j] = part.load(part.v0 + j * THREADS + threadIdx.x);
+    for (uint32_t s = part.v0; s < part.v1; s += kStep) {
         float f[kLpPer];
-        bool in = true;  // every value of this thread's pieces is one of the row
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const uint32_t v = s + j * kLpThreads + threadIdx.x;
-            const int64_t e0 = (int64_t)v * VE - off;
-            if (v < v1 && e0 >= 0 && e0 + VE <= (int64_t)p.vocab) {
-                const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(base) + v);
-                const T *t = reinterpret_cast<const T *>(&u);
+        for (int j = 0; j < NV; j++) Part::values(next[j], f + j * VE);
+        if (s + kStep < part.v1) {
 #pragma unroll
-                for (int i = 0; i < VE; i++) f[j * VE + i] = to_f32(t[i]);
-            } else {
-                in = false;
-#pragma unroll
-                for (int i = 0; i < VE; i++)
-                    f[j * VE + i] = v < v1 && e0 + i >= 0 && e0 + i < (int64_t)p.vocab ? to_f32(x[e0 + i]) : -INFINITY;
-            }
+            for (int j = 0; j < NV; j++) next[j] = part.load(s + kStep + j * THREADS + threadIdx.x);
         }
-        float c = f[0];
+        float c[4] = {f[0], f[1], f[2], f[3]};
 #pragma unroll
-        for (int i = 1; i < kLpPer; i++) c = fmaxf(c, f[i]);
-        if (c > a.m) a.raise(c);
+        for (int i = 4; i < kLpPer; i++) c[i & 3] = fmaxf(c[i & 3], f[i]);
+        const float top = fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3]));
+        if (top > a.m) a.raise(top);
         if (a.m != -INFINITY) {
+            LpSum b{a.m};  // two chains
 #pragma unroll
-            for (int i = 0; i < kLpPer; i++) a.add(f[i]);
+            for (int i = 0; i < kLpPer; i += 2) a.add(f[i]), b.add(f[i + 1]);
+            a.z += b.z, a.w += b.w;
         } else {  // nothing above -inf so far: only a NaN counts
 #pragma unroll
             for (int i = 0; i < kLpPer; i++)
                 if (f[i] != f[i]) a.z = f[i];
         }
         if (k == 0) continue;
-        auto index = [&](int i) {  // of value i, below vocab
-            return (uint32_t)((int64_t)(s + (i / VE) * kLpThreads + threadIdx.x) * VE - off + i % VE);
-        };
-        auto valid = [&](int i) { return in || (s + (i / VE) * kLpThreads + threadIdx.x < v1 && index(i) < p.vocab); };
-        if (s == v0) {
+        auto piece = [&](int i) { return s + (i / VE) * THREADS + threadIdx.x; };
+        if (done == 0) {
             uint64_t mx = 0;
 #pragma unroll
             for (int i = 0; i < kLpPer; i++) {
-                const uint64_t key = valid(i) ? lp_key(f[i], index(i)) : 0;
+                const uint64_t key = part.valid(piece(i), i % VE) ? lp_key(f[i], part.index(piece(i), i % VE)) : 0;
                 mx = key > mx ? key : mx;
             }
             bound = lp_bound(sm, mx, k);
-            if (bound) boundf = lp_value((uint32_t)(bound >> 32));
+        } else if ((done & (done - 1)) == 0 && done > 1) {  // 2, 4, 8, ... steps are in the list
+            __syncthreads();
+            const uint32_t n = sm.n;
+            __syncthreads();
+            if (n > 2 * k && n <= (uint32_t)kLpCap) bound = lp_compact(sm, n, k);
         }
+        done++;
+        boundf = bound ? lp_value((uint32_t)(bound >> 32)) : -INFINITY;
         bool any = false;
 #pragma unroll
         for (int i = 0; i < kLpPer; i++) any |= !(f[i] < boundf);
         if (any) {
 #pragma unroll
             for (int i = 0; i < kLpPer; i++)
-                if (!(f[i] < boundf) && valid(i)) {
-                    const uint64_t key = lp_key(f[i], index(i));
-                    if (key >= bound) sm.cand[atomicAdd(&sm.n, 1u)] = key;
+                if (!(f[i] < boundf) && part.valid(piece(i), i % VE)) {
+                    const uint64_t key = lp_key(f[i], part.index(piece(i), i % VE));
+                    if (key >= bound) {
+                        const uint32_t at = atomicAdd(&sm.n, 1u);
+                        if (at < (uint32_t)kLpCap) sm.cand[at] = key;
+                    }
                 }
         }
+    }
+    if (k > 0) {
         __syncthreads();
-        uint32_t n = sm.n;
-        __syncthreads();
-        while (n > (uint32_t)kLpKeep) {  // at most k * ceil(n / 256) <= n / 2 + 128 keys stay
-            bound = lp_compact(sm, n, k);
-            boundf = bound ? lp_value((uint32_t)(bound >> 32)) : -INFINITY;
-            n = sm.n;
-            __syncthreads();
-        }
+        if (sm.n > (uint32_t)kLpCap) lp_checked<T, THREADS>(sm, part, k);
     }
     // ---- join the threads' sums ----
 #pragma unroll
@@ -212,15 +280,15 @@ __global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, 
     __syncthreads();
     if (threadIdx.x == 0) {
         LpSum t{sm.rm[0], sm.rz[0], sm.rw[0]};
-        for (int i = 1; i < kLpThreads / 32; i++) t.join(sm.rm[i], sm.rz[i], sm.rw[i]);
+        for (int i = 1; i < THREADS / 32; i++) t.join(sm.rm[i], sm.rz[i], sm.rw[i]);
         sm.cm = t.m, sm.cz = t.z, sm.cw = t.w;
     }
     // ---- this CTA's largest keys, in order ----
     if (k > 0) {
-        for (uint32_t i = threadIdx.x; i < k; i += kLpThreads) sm.top[i] = 0;
+        for (uint32_t i = threadIdx.x; i < k; i += THREADS) sm.top[i] = 0;
         __syncthreads();
         const uint32_t n = sm.n;
-        for (uint32_t i = threadIdx.x; i < n; i += kLpThreads) {
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
             const uint64_t key = sm.cand[i];
             uint32_t above = 0;
             for (uint32_t j = 0; j < n; j++) above += sm.cand[j] > key;
@@ -238,18 +306,18 @@ __global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, 
                 sm.rm[0] = t.m, sm.rz[0] = t.z, sm.rw[0] = t.w;
             }
             const uint32_t n = splits * k;  // <= 2048
-            for (uint32_t i = threadIdx.x; i < n; i += kLpThreads) {
+            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
                 const uint32_t src = cluster_addr(smem_u32(&sm.top[i % k]), i / k);
                 uint64_t key;
                 asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(src) : "memory");
                 sm.cand[i] = key;
             }
             __syncthreads();
-            uint64_t keys[kLpMaxTop * kLpMaxSplits / kLpThreads];
-            uint32_t ranks[kLpMaxTop * kLpMaxSplits / kLpThreads];
+            uint64_t keys[kLpMaxTop * kLpMaxSplits / THREADS];
+            uint32_t ranks[kLpMaxTop * kLpMaxSplits / THREADS];
 #pragma unroll
-            for (int q = 0; q < kLpMaxTop * kLpMaxSplits / kLpThreads; q++) {
-                const uint32_t i = threadIdx.x + q * kLpThreads;
+            for (int q = 0; q < kLpMaxTop * kLpMaxSplits / THREADS; q++) {
+                const uint32_t i = threadIdx.x + q * THREADS;
                 keys[q] = i < n ? sm.cand[i] : 0;
                 uint32_t above = 0;
                 if (keys[q])
@@ -258,7 +326,7 @@ __global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, 
             }
             __syncthreads();
 #pragma unroll
-            for (int q = 0; q < kLpMaxTop * kLpMaxSplits / kLpThreads; q++)
+            for (int q = 0; q < kLpMaxTop * kLpMaxSplits / THREADS; q++)
                 if (keys[q] && ranks[q] < k) sm.cand[ranks[q]] = keys[q];
             __syncthreads();
         }
@@ -284,18 +352,22 @@ __global__ void __launch_bounds__(kLpThreads) k_logprobs(const LogprobParams p, 
         }
     }
     const uint64_t *top = splits > 1 ? sm.cand : sm.top;
-    for (uint32_t i = threadIdx.x; i < k; i += kLpThreads) {
+    for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
         const uint64_t key = top[i];
         p.top_ids[(uint64_t)r * k + i] = (int32_t)~(uint32_t)key;
         p.top_logprobs[(uint64_t)r * k + i] = lp_value((uint32_t)(key >> 32)) - m - lz;
     }
 }
 
+template <typename T, int THREADS>
+static int launch_lp_threads(rcu_ctx *ctx, const LogprobParams &p, uint32_t per_sm) {
+    uint32_t cs = 1;  // up to per_sm CTAs for each SM, and no CTA without a step's values
+    while (cs < kLpMaxSplits && (uint64_t)p.rows * cs * 2 <= (uint64_t)per_sm * ctx->num_sms && p.vocab >= (uint64_t)cs * THREADS * kLpPer) cs *= 2;
+    return launch_cluster_k(ctx, k_logprobs<T, THREADS>, p.rows * cs, THREADS, sizeof(LpSmem), cs, p, cs);
+}
 template <typename T>
 static int launch_lp(rcu_ctx *ctx, const LogprobParams &p) {
-    uint32_t cs = 1;  // up to four CTAs for each SM, two steps of values for each
-    while (cs < kLpMaxSplits && (uint64_t)p.rows * cs * 2 <= 4ull * ctx->num_sms && p.vocab >= (uint64_t)cs * 2 * kLpStep) cs *= 2;
-    return launch_cluster_k(ctx, k_logprobs<T>, p.rows * cs, kLpThreads, sizeof(LpSmem), cs, p, cs);
+    return p.rows <= 4 ? launch_lp_threads<T, 1024>(ctx, p, 1) : launch_lp_threads<T, 256>(ctx, p, 4);
 }
 
 int launch_logprobs(rcu_ctx *ctx, const LogprobParams &p, int type) {

@@ -21,8 +21,30 @@ struct rcu_paged {
 
 namespace rcu {
 
-// One warp per (new token, k or v): the warp finds its token's sequence (rows cu[i + 1] <= t are
-// counted, 32 sequences a step) and rounds the row to f16 once, 8 values a lane and step.
+// Eight values rounded to f16.
+template <typename T>
+struct Eight {
+    uint4 a, b;  // as loaded (f32: two pieces)
+    __device__ __forceinline__ void load(const T *p) {
+        a = __ldcs(reinterpret_cast<const uint4 *>(p));
+        if constexpr (sizeof(T) == 4) b = __ldcs(reinterpret_cast<const uint4 *>(p) + 1);
+    }
+    __device__ __forceinline__ uint4 half8() const {
+        if constexpr (sizeof(T) == 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(&a), y = *reinterpret_cast<const float4 *>(&b);
+            return make_uint4(pack2<__half>(x.x, x.y), pack2<__half>(x.z, x.w), pack2<__half>(y.x, y.y), pack2<__half>(y.z, y.w));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            return a;
+        } else {
+            const float2 x = unpack2<T>(a.x), y = unpack2<T>(a.y), z = unpack2<T>(a.z), w = unpack2<T>(a.w);
+            return make_uint4(pack2<__half>(x.x, x.y), pack2<__half>(y.x, y.y), pack2<__half>(z.x, z.y), pack2<__half>(w.x, w.y));
+        }
+    }
+};
+
+// One warp per (new token, k or v), 8 values a lane and step. The row's first values are on their way
+// before the warp looks up where they go (its sequence: rows cu[i + 1] <= t are counted, 32 sequences
+// a step; then length and page, one after the other): bound by bytes, if enough of them are in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) k_paged_store(const SeqView b, const T *__restrict__ k, const T *__restrict__ v,
                                                      uint64_t ld, uint32_t n_kv, uint32_t hd, __half *kp, __half *vp) {
@@ -30,6 +52,13 @@ __global__ void __launch_bounds__(256) k_paged_store(const SeqView b, const T *_
     pdl_trigger();
     const uint32_t lane = threadIdx.x & 31, w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), t = w >> 1;
     if (t >= b.n_tok) return;
+    constexpr int kAhead = 4;
+    const T *src = (w & 1 ? v : k) + (uint64_t)t * ld;
+    const uint32_t vecs = n_kv * hd / 8, per = hd / 8;
+    Eight<T> x[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++)
+        if (lane + 32 * j < vecs) x[j].load(src + 8 * (lane + 32 * j));
     uint32_t seq = 0;
     for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 32)
         seq += __popc(__ballot_sync(0xffffffffu, s0 + lane < b.n_seq && b.cu[s0 + lane + 1] <= (int32_t)t));
@@ -42,29 +71,21 @@ __global__ void __launch_bounds__(256) k_paged_store(const SeqView b, const T *_
     const uint32_t pg = seq_page(b, seq, (uint32_t)(pos >> b.page_shift));
     if (pg == kNoRow) return;
     const uint32_t ps = 1u << b.page_shift, slot = (uint32_t)pos & (ps - 1);
-    const T *src = (w & 1 ? v : k) + (uint64_t)t * ld;
     __half *dst = w & 1 ? vp : kp;
-    const uint32_t vecs = n_kv * hd / 8, per = hd / 8;
-#pragma unroll 4
-    for (uint32_t i = lane; i < vecs; i += 32) {
-        uint4 o;
-        if constexpr (sizeof(T) == 4) {
-            const float4 x0 = *reinterpret_cast<const float4 *>(src + 8 * i), x1 = *reinterpret_cast<const float4 *>(src + 8 * i + 4);
-            o = make_uint4(pack2<__half>(x0.x, x0.y), pack2<__half>(x0.z, x0.w), pack2<__half>(x1.x, x1.y), pack2<__half>(x1.z, x1.w));
-        } else {
-            o = *reinterpret_cast<const uint4 *>(src + 8 * i);
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                uint32_t *e = reinterpret_cast<uint32_t *>(&o);
+    for (uint32_t i0 = 0; i0 < vecs; i0 += 32 * kAhead) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float2 x = unpack2<__nv_bfloat16>(e[j]);
-                    e[j] = pack2<__half>(x.x, x.y);
-                }
-            }
+        for (int j = 0; j < kAhead; j++) {
+            const uint32_t i = i0 + 32 * j + lane;
+            if (i >= vecs) continue;
+            const uint32_t h = i / per, c = i - h * per;
+            const uint64_t row = ((uint64_t)pg * n_kv + h) * ps + slot;
+            *reinterpret_cast<uint4 *>(dst + row * hd + 8 * c) = x[j].half8();
         }
-        const uint32_t h = i / per, c = i - h * per;
-        const uint64_t row = ((uint64_t)pg * n_kv + h) * ps + slot;
-        *reinterpret_cast<uint4 *>(dst + row * hd + 8 * c) = o;
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const uint32_t i = i0 + 32 * (kAhead + j) + lane;
+            if (i < vecs) x[j].load(src + 8 * i);
+        }
     }
 }
 
