@@ -382,10 +382,23 @@ def attention(ctx: Context, cache: LayerCache, q, n_tok: int, n_head: int, pos0:
                                            float(softcap or 0.0), C.c_void_p(_dptr(out))))
 
 
-def _elem(x) -> GgmlType:
+_ELEM: dict = {}   # torch dtype -> GGUF type id
+_DTYPE: dict = {}  # name -> torch dtype
+
+
+def _torch_types() -> None:
+    import torch
+    _ELEM.update({torch.float32: int(GgmlType.F32), torch.float16: int(GgmlType.F16), torch.bfloat16: int(GgmlType.BF16)})
+    _DTYPE.update(f32=torch.float32, i32=torch.int32)
+
+
+def _elem(x) -> int:
     """GGUF type id of a tensor's elements."""
-    ty = {"torch.float32": GgmlType.F32, "torch.float16": GgmlType.F16, "torch.bfloat16": GgmlType.BF16}.get(str(x.dtype))
+    ty = _ELEM.get(x.dtype)
     if ty is None:
+        if not _ELEM:
+            _torch_types()
+            return _elem(x)
         raise ValueError(f"f32, f16 or bf16 values expected, not {x.dtype}")
     return ty
 
@@ -402,15 +415,18 @@ def _on(ctx: Context, x, what: str) -> int:
 def _rows(ctx: Context, x, n: int, width: int, what: str):
     """(address, type, row stride) of n rows of `width` values; the rows may be slices of wider
     ones, their values must be contiguous."""
-    if x.dim() != 2 or x.shape[0] != n or x.shape[1] != width:
+    if x.shape != (n, width):
         raise ValueError(f"{what}: expected {n} x {width} values, not {tuple(x.shape)}")
-    if x.stride(1) != 1 and width > 1:
+    ld, step = x.stride()
+    if step != 1 and width > 1:
         raise ValueError(f"{what}: the values of a row must be contiguous")
-    return _on(ctx, x, what), _elem(x), x.stride(0) if n > 1 else max(x.stride(0), width)
+    return _on(ctx, x, what), _elem(x), ld if n > 1 else max(ld, width)
 
 
 def _vector(ctx: Context, x, dtype: str, shape, what: str) -> int:
-    if str(x.dtype) != dtype or tuple(x.shape) != tuple(shape) or not x.is_contiguous():
+    if not _DTYPE:
+        _torch_types()
+    if x.dtype is not _DTYPE[dtype] or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, not {x.dtype} {tuple(x.shape)}")
     return _on(ctx, x, what)
 
@@ -521,7 +537,7 @@ def packed_attention(ctx: Context, q, k, v, cu, n_head: int, n_head_kv: int, hea
         raise ValueError("k and v must have the same type and row stride, q and out the same type")
     n_seq = cu.shape[0] - 1
     _check(ctx.ptr, ctx._lib.rcu_packed_attention(ctx.ptr, qp, ty, ld, kp, vp, ty_k, ld_k,
-                                                  _vector(ctx, cu, "torch.int32", (n_seq + 1,), "cu"), n_seq, n_tok,
+                                                  _vector(ctx, cu, "i32", (n_seq + 1,), "cu"), n_seq, n_tok,
                                                   max_len, n_head, n_head_kv, head_dim, window, softcap or 0.0, op, ld_o))
 
 
@@ -540,11 +556,11 @@ def logprobs(ctx: Context, logits, targets=None, logprob=None, entropy=None, top
     def arg(x, dtype, shape, what):
         return None if x is None else _vector(ctx, x, dtype, shape, what)
 
-    ids = arg(top_ids, "torch.int32", (n, top_k), "top_ids")
-    tlp = arg(top_logprobs, "torch.float32", (n, top_k), "top_logprobs")
-    _check(ctx.ptr, ctx._lib.rcu_logprobs(ctx.ptr, lp, ty, n, width, ld, arg(targets, "torch.int32", (n,), "targets"),
-                                          arg(logprob, "torch.float32", (n,), "logprob"),
-                                          arg(entropy, "torch.float32", (n,), "entropy"), top_k, ids if top_k else None,
+    ids = arg(top_ids, "i32", (n, top_k), "top_ids")
+    tlp = arg(top_logprobs, "f32", (n, top_k), "top_logprobs")
+    _check(ctx.ptr, ctx._lib.rcu_logprobs(ctx.ptr, lp, ty, n, width, ld, arg(targets, "i32", (n,), "targets"),
+                                          arg(logprob, "f32", (n,), "logprob"),
+                                          arg(entropy, "f32", (n,), "entropy"), top_k, ids if top_k else None,
                                           tlp if top_k else None))
 
 

@@ -35,7 +35,7 @@
 
 namespace rcu {
 
-constexpr int kSqKeys = 16;     // keys of a chunk
+constexpr int kSqKeys = kSeqFewBox;  // keys of a chunk
 constexpr int kSqWarps = 4;
 constexpr int kSqStages = 2;  // three CTAs to an SM; with three stages two, of which clusters of 16 leave SMs idle (199 against 159 us)
 constexpr int kSqMaxCluster = 16;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
 
 // ---- host ---------------------------------------------------------------------------------------
 template <typename T, typename E, int HDP, int NT>
-static int launch_few(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv, SeqAttnParams p, uint64_t max_len) {
+static int launch_few(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64_t max_len) {
     const size_t smem = sizeof(SqSmem<HDP>) + 1024;
     p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, (std::is_same<T, float>::value ? 4 : 8) * NT);
     // CTAs per tile: up to three for each SM in all, and at least 128 keys each
@@ -429,22 +429,23 @@ static int launch_few(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv
     while (cs < most && items * cs * 2 <= 3ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 128) cs *= 2;
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
-    return launch_cluster_k(ctx, k_attn_seq<T, E, HDP, NT>, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, mk, mv, p);
+    return launch_cluster_k<k_attn_seq<T, E, HDP, NT>>(ctx, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, m.k, m.v, p);
 }
 
 // One fragment of rows where they fill no more (a group's heads for single tokens), else two.
 template <typename T, typename E>
 static int launch_few_hd(rcu_ctx *ctx, const SeqAttnParams &p, const SeqKvDesc &kv, uint64_t max_len, uint64_t most) {
-    CUtensorMap mk, mv;
-    if (int st = seq_kv_maps(ctx, p, kv, kSqKeys, &mk, &mv)) return st;
+    SeqKvMaps room;
+    const SeqKvMaps *m;
+    if (int st = seq_pick_maps(ctx, p, kv, kSeqFewBox, kv.few, &room, &m)) return st;
     if (most <= (std::is_same<T, float>::value ? 4u : 8u)) {
-        if (p.hd <= 64) return launch_few<T, E, 64, 1>(ctx, mk, mv, p, max_len);
-        if (p.hd <= 128) return launch_few<T, E, 128, 1>(ctx, mk, mv, p, max_len);
-        return launch_few<T, E, 256, 1>(ctx, mk, mv, p, max_len);
+        if (p.hd <= 64) return launch_few<T, E, 64, 1>(ctx, *m, p, max_len);
+        if (p.hd <= 128) return launch_few<T, E, 128, 1>(ctx, *m, p, max_len);
+        return launch_few<T, E, 256, 1>(ctx, *m, p, max_len);
     }
-    if (p.hd <= 64) return launch_few<T, E, 64, 2>(ctx, mk, mv, p, max_len);
-    if (p.hd <= 128) return launch_few<T, E, 128, 2>(ctx, mk, mv, p, max_len);
-    return launch_few<T, E, 256, 2>(ctx, mk, mv, p, max_len);
+    if (p.hd <= 64) return launch_few<T, E, 64, 2>(ctx, *m, p, max_len);
+    if (p.hd <= 128) return launch_few<T, E, 128, 2>(ctx, *m, p, max_len);
+    return launch_few<T, E, 256, 2>(ctx, *m, p, max_len);
 }
 
 static int launch_attention_few(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,

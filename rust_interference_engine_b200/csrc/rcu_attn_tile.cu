@@ -31,7 +31,7 @@
 namespace rcu {
 
 constexpr int kTlRows = 256;       // query rows per CTA (two tiles)
-constexpr int kTlBlk = 128;        // keys per block
+constexpr int kTlBlk = kSeqTileBox;  // keys per block
 constexpr int kTlSoftWarps = 16;
 constexpr int kTlThreads = 640;    // four softmax warpgroups; a fifth for the producer and the MMA issuer
 // registers a thread: the fifth warpgroup gives its own up (4 x 112 + 32 = 5 x 96, the launch's)
@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
 bool attention_tile_ok(uint64_t hd) { return hd <= 128; }
 
 template <typename T, typename E, int HDP>
-static int launch_tile(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &mv, SeqAttnParams p, uint64_t max_len) {
+static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64_t max_len) {
     constexpr size_t smem = sizeof(TlSmem<HDP, std::is_same<T, float>::value>);
     static_assert(smem <= 232448, "shared memory of one CTA");
     const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + kTlRows) : max_len;
@@ -710,16 +710,16 @@ static int launch_tile(rcu_ctx *ctx, const CUtensorMap &mk, const CUtensorMap &m
     while (cs < kTlMaxCluster && items * cs * 2 <= (uint64_t)ctx->num_sms && span >= (uint64_t)cs * 2 * 4 * kTlBlk) cs *= 2;
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
-    return launch_cluster_k(ctx, k_attn_tile<T, E, HDP>, (uint32_t)(items * cs), kTlThreads, smem, cs, mk, mv, p);
+    return launch_cluster_k<k_attn_tile<T, E, HDP>>(ctx, (uint32_t)(items * cs), kTlThreads, smem, cs, m.k, m.v, p);
 }
 
 template <typename T, typename E>
 static int launch_tile_hd(rcu_ctx *ctx, SeqAttnParams &p, const SeqKvDesc &kv, uint64_t max_len) {
-    CUtensorMap mk, mv;
-    const uint32_t box = kv.pages ? std::min<uint32_t>(1u << p.b.page_shift, kTlBlk) : kTlBlk;
-    if (int st = seq_kv_maps(ctx, p, kv, box, &mk, &mv)) return st;
+    SeqKvMaps room;
+    const SeqKvMaps *m;
+    if (int st = seq_pick_maps(ctx, p, kv, kSeqTileBox, kv.tile, &room, &m)) return st;
     p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kTlRows);
-    return p.hd <= 64 ? launch_tile<T, E, 64>(ctx, mk, mv, p, max_len) : launch_tile<T, E, 128>(ctx, mk, mv, p, max_len);
+    return p.hd <= 64 ? launch_tile<T, E, 64>(ctx, *m, p, max_len) : launch_tile<T, E, 128>(ctx, *m, p, max_len);
 }
 
 int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &params, int q_type, const SeqKvDesc &kv, uint64_t max_len) {

@@ -121,10 +121,12 @@ uint64_t attention_scratch_bytes_upto(const rcu_ctx *ctx, const rcu_kv *kv, uint
 // read, rows of hd elements: the page pool's rows [page][kv head][slot], or packed prompt rows with
 // a stride between kv heads. max_len shapes the launch only.
 struct SeqAttnParams;
+struct SeqKvMaps;
 struct SeqKvDesc {
     const void *k, *v;
     bool pages;
     uint64_t rows, row_stride, head_stride;  // strides in elements
+    const SeqKvMaps *few, *tile;  // a pool's tensor maps for the two kernels; nullptr: made for the call
 };
 // (max_new too: 0 when unknown). q_type T_F32 or T_F16 over f16, or T_BF16 over bf16.
 int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,
@@ -132,6 +134,7 @@ int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const
 // Its kernel for sequences of many query rows per KV head (rcu_attn_tile.cu), head_dim <= 128.
 constexpr uint32_t kTileMinRows = 64;
 bool attention_tile_ok(uint64_t hd);
+constexpr uint32_t kSeqFewBox = 16, kSeqTileBox = 128;  // rows of a load: kSeqFewBox; a page's, kSeqTileBox at most
 int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len);
 // log p of targets, entropy and the largest top_k of rows of logits (rcu_logprobs.cu).
 struct LogprobParams {

@@ -479,7 +479,7 @@ static int launch_lp_threads(rcu_ctx *ctx, const LogprobParams &p, uint32_t per_
         const uint64_t cost = ((uint64_t)p.rows * c + slots - 1) / slots * (p.vocab / c + 8192);
         if (cost < best) best = cost, cs = c;
     }
-    return launch_cluster_k(ctx, k_logprobs<T, THREADS>, p.rows * cs, THREADS, lp_smem<THREADS>(), cs, p, cs);
+    return launch_cluster_k<k_logprobs<T, THREADS>>(ctx, p.rows * cs, THREADS, lp_smem<THREADS>(), cs, p, cs);
 }
 template <typename T>
 static int launch_lp(rcu_ctx *ctx, const LogprobParams &p) {

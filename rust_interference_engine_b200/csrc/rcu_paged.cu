@@ -17,6 +17,7 @@ struct rcu_paged {
     uint32_t page_shift = 0;
     void *k = nullptr, *v = nullptr;
     bool owned = false;
+    rcu::SeqKvMaps few, tile;  // boxes of 16 rows, and of a page's rows (128 at most)
 };
 
 namespace rcu {
@@ -169,6 +170,13 @@ int32_t rcu_paged_create(rcu_ctx *ctx, int32_t kv_type, uint64_t n_head_kv, uint
             return cuda_err(ctx, e, "paged cache alloc");
         }
     }
+    const SeqKvDesc kv{pg->k, pg->v, true, n_pages * n_head_kv * page_size, head_dim, head_dim, nullptr, nullptr};
+    int st = seq_kv_maps(ctx, kv, head_dim, n_head_kv, kSeqFewBox, &pg->few);
+    if (!st) st = seq_kv_maps(ctx, kv, head_dim, n_head_kv, (uint32_t)std::min<uint64_t>(page_size, kSeqTileBox), &pg->tile);
+    if (st) {
+        rcu_paged_free(pg);
+        return st;
+    }
     *out = pg;
     return RCU_OK;
     RCU_GUARD_END(ctx)
@@ -241,7 +249,7 @@ int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s
     p.softcap = softcap;
     const uint64_t cap = seqs->ld_pages * pg->page_size;
     DeviceGuard guard(ctx);
-    const SeqKvDesc kv{pg->k, pg->v, true, p.kv_rows, pg->hd, pg->hd};
+    const SeqKvDesc kv{pg->k, pg->v, true, p.kv_rows, pg->hd, pg->hd, &pg->few, &pg->tile};
     return launch_seq_attention(ctx, p, (int)type, kv, seqs->max_len ? std::min(seqs->max_len, cap) : cap, seqs->max_new);
     RCU_GUARD_END(ctx)
 }
@@ -279,7 +287,7 @@ int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, u
     p.window = (uint32_t)window;
     p.softcap = softcap;
     DeviceGuard guard(ctx);
-    const SeqKvDesc kv{k_dev, v_dev, false, n_tok, ld_kv, head_dim};
+    const SeqKvDesc kv{k_dev, v_dev, false, n_tok, ld_kv, head_dim, nullptr, nullptr};
     return launch_seq_attention(ctx, p, (int)q_type, kv, max_len ? std::min(max_len, n_tok) : n_tok, max_len);
     RCU_GUARD_END(ctx)
 }

@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "rcu_kernels.h"
 #include "rcu_tc.cuh"
@@ -288,21 +289,37 @@ __device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan 
 
 // ---- host ---------------------------------------------------------------------------------------
 // Tensor maps of k and v with boxes of `box` rows of 64 elements (128-byte swizzle).
-inline int seq_kv_maps(rcu_ctx *ctx, const SeqAttnParams &p, const SeqKvDesc &kv, uint32_t box, CUtensorMap *mk, CUtensorMap *mv) {
+struct SeqKvMaps {
+    CUtensorMap k, v;
+};
+inline int seq_kv_maps(rcu_ctx *ctx, const SeqKvDesc &kv, uint64_t hd, uint64_t n_kv, uint32_t box, SeqKvMaps *m) {
     for (int i = 0; i < 2; i++)
-        if (int st = make_map_3d(ctx, i ? mv : mk, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? kv.v : kv.k, p.hd, kv.pages ? 1 : p.n_kv,
+        if (int st = make_map_3d(ctx, i ? &m->v : &m->k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, i ? kv.v : kv.k, hd, kv.pages ? 1 : n_kv,
                                  kv.rows, kv.head_stride * 2, kv.row_stride * 2, 64, 1, box, CU_TENSOR_MAP_SWIZZLE_128B))
             return st;
     return RCU_OK;
 }
-// Clusters of cs CTAs, programmatic dependent launch as launch_k.
-template <typename... KArgs, typename... Args>
-inline int launch_cluster_k(rcu_ctx *ctx, void (*kern)(KArgs...), uint32_t grid, uint32_t threads, size_t smem, uint32_t cs,
-                            const Args &...args) {
-    const void *fn = reinterpret_cast<const void *>(kern);
-    RCU_CUDA_TRY(ctx, prefer_max_shared(fn));
-    RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (cs > 8) RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+// The maps that a launch with boxes of `box` rows uses: the pool's own, made with it, or new ones.
+inline int seq_pick_maps(rcu_ctx *ctx, const SeqAttnParams &p, const SeqKvDesc &kv, uint32_t box, const SeqKvMaps *made,
+                         SeqKvMaps *room, const SeqKvMaps **use) {
+    *use = made;
+    if (made) return RCU_OK;
+    *use = room;
+    return seq_kv_maps(ctx, kv, p.hd, p.n_kv, box, room);
+}
+// Clusters of cs CTAs, programmatic dependent launch as launch_k. The kernel's attributes are set by
+// its first launch on a device.
+template <auto Kern, typename... Args>
+inline int launch_cluster_k(rcu_ctx *ctx, uint32_t grid, uint32_t threads, size_t smem, uint32_t cs, const Args &...args) {
+    static std::atomic<uint64_t> ready{0};  // devices, of the first 64
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (ctx->device >= 64 || !(ready.load(std::memory_order_acquire) & bit)) {
+        const void *fn = reinterpret_cast<const void *>(Kern);
+        RCU_CUDA_TRY(ctx, prefer_max_shared(fn));
+        RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        ready.fetch_or(bit, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
@@ -323,7 +340,7 @@ inline int launch_cluster_k(rcu_ctx *ctx, void (*kern)(KArgs...), uint32_t grid,
     }
     cfg.attrs = attr;
     cfg.numAttrs = na;
-    RCU_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, args...));
+    RCU_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, Kern, args...));
     return RCU_OK;
 }
 
