@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
     __syncwarp();
     const uint32_t row0 = tile * kRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kRows);
     // the tile's attended positions k_lo .. k_hi; positions stay below 2^31
-    const int32_t p_first = (int32_t)sp.pos(row0 / p.group), k_hi = (int32_t)sp.pos((row0 + n_rows - 1) / p.group);
+    const int32_t p_first = sp.pos(div_group(p, row0)), k_hi = sp.pos(div_group(p, row0 + n_rows - 1));
     const int32_t k_lo = p.window > 0 ? max(p_first - (int32_t)p.window + 1, 0) : 0;
     const uint32_t c_lo = (uint32_t)(k_lo / kSqKeys), c_all = k_hi >= 0 ? (uint32_t)(k_hi / kSqKeys) + 1 : 0;
     const uint32_t n_chunks = c_all > c_lo ? c_all - c_lo : 0;
@@ -160,8 +160,9 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
     for (int n = 0; n < NT; n++) {
         const uint32_t r = kPer * n + g % kPer, rr = row0 + min(r, n_rows - 1);
         const bool live = r < n_rows;
-        const T *src = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + rr / p.group) * p.ld_q +
-                       (uint64_t)(kvh * p.group + rr % p.group) * p.hd;
+        const uint32_t tok = div_group(p, rr);
+        const T *src = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + tok) * p.ld_q +
+                       (uint64_t)(kvh * p.group + rr - tok * p.group) * p.hd;
         if constexpr (kSplit) {
             float2 x[KS][2];
             float mx = 0.0f;
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const uint32_t r = kPer * n + (2 * t4 + i) % kPer;
-            shi[n][i] = r < n_rows ? (int32_t)sp.pos((row0 + r) / p.group) : -1;
+            shi[n][i] = r < n_rows ? sp.pos(div_group(p, row0 + r)) : -1;
             slo[n][i] = p.window > 0 ? max(shi[n][i] - (int32_t)p.window + 1, 0) : 0;
         }
     float o[NT][KS][4];  // O^T: columns 16 ks + g (+ 8) of rows as the scores' (f32: high parts, the rest)
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
                 for (int i = 0; i < HDP / 32; i++) acc[i] = fmaf(w, ld_cluster_f32(a + 128 * i), acc[i]);
             }
         }
-        const uint32_t rr = row0 + r, t = rr / p.group, gq = rr % p.group;
+        const uint32_t rr = row0 + r, t = div_group(p, rr), gq = rr - t * p.group;
         T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + t) * p.ld_out + (uint64_t)(kvh * p.group + gq) * p.hd;
         bool fine = true;
 #pragma unroll

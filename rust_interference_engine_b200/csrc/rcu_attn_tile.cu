@@ -97,6 +97,11 @@ __device__ __forceinline__ void tl_tmem_st16(uint32_t taddr, const uint32_t (&v)
         "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
+__device__ __forceinline__ void tl_tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ void tl_tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -134,10 +139,9 @@ struct TlSpan {
     int32_t lo, hi;
 };
 __device__ __forceinline__ TlSpan tl_span(const SeqAttnParams &p, const SeqSpan &sp, uint32_t r0, uint32_t r1) {
-    const int64_t a = sp.pos(r0 / p.group), b = sp.pos((r1 - 1) / p.group);
+    const int32_t a = sp.pos(div_group(p, r0)), b = sp.pos(div_group(p, r1 - 1));
     if (b < 0) return {0, 0};
-    const int64_t lo = p.window > 0 && a + 1 > (int64_t)p.window ? a + 1 - p.window : 0;
-    return {(int32_t)(lo / kTlBlk), (int32_t)(b / kTlBlk) + 1};
+    return {p.window > 0 ? max(a - (int32_t)p.window + 1, 0) / kTlBlk : 0, b / kTlBlk + 1};
 }
 
 template <typename T, typename E, int HDP>
@@ -196,8 +200,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             const uint32_t w8 = warp & 7;
             auto source = [&](uint32_t i) {  // row i of the tile
                 const uint32_t rr = row0 + min(128 * t + i, n_rows - 1);
-                return reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + rr / p.group) * p.ld_q +
-                       (uint64_t)(kvh * p.group + rr % p.group) * p.hd;
+                const uint32_t tk = div_group(p, rr);
+                return reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + tk) * p.ld_q +
+                       (uint64_t)(kvh * p.group + rr - tk * p.group) * p.hd;
             };
             if constexpr (kSplit) {
                 constexpr int kLanes = HDP / 4, kPer = 32 / kLanes;  // lanes of a row (4 values each), rows a warp and step
@@ -268,14 +273,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         bool met = false;
         const uint32_t box = p.b.pages ? min(1u << p.b.page_shift, (uint32_t)kTlBlk) : (uint32_t)kTlBlk;
         const uint32_t n_box = kTlBlk / box;  // boxes of rows per block (8 at most, pages of 16)
-        const int64_t end = sp.pos((row0 + n_rows - 1) / p.group) + 1;
+        const int32_t end = sp.pos(div_group(p, row0 + n_rows - 1)) + 1;
         uint32_t it = 0;
         bool ok = true;
         for (int32_t j = j0; j < j1 && ok; j++) {
             if (it + 2 > C::kStages && !met) met = true, meet();
             // lane l < n_box * kChunks brings box l % n_box of 64-element chunk l / n_box
             const uint32_t bx = lane % n_box, ch = lane / n_box;
-            const int64_t pos = (int64_t)j * kTlBlk + bx * box;
+            const int32_t pos = j * kTlBlk + (int32_t)(bx * box);
             uint32_t row = p.kv_rows;  // behind the tensor: zeros
             if (ch < kChunks && pos < end) row = min(seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)pos), p.kv_rows);
 #pragma unroll
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         auto uni = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
         const int32_t n_blk = uni(j1 - j0), b0 = uni(jb[0] - j0), e0 = uni(je[0] - j0), b1 = uni(jb[1] - j0), e1 = uni(je[1] - j0);
         // keys from this CTA's first block to the last one that a row attends
-        const int32_t n_keys = uni((int32_t)(sp.pos((row0 + n_rows - 1) / p.group) + 1 - (int64_t)j0 * kTlBlk));
+        const int32_t n_keys = uni(sp.pos(div_group(p, row0 + n_rows - 1)) + 1 - j0 * kTlBlk);
         const uint32_t tm = uni((int32_t)tmem);
         const uint64_t dq = sw128_desc(sm.data), dk = sw128_desc(ring), dv = sw128_desc_mn(ring, kTlBlk * 128);
         const bool elected = elect_one();
@@ -395,15 +400,15 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         const uint32_t lanes = (32 * (warp & 3)) << 16;  // their TMEM lanes
         const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 256 + HDP * t + HDP / 2 * h + lanes;
         const bool live = tr < n_rows;
-        const uint32_t row = row0 + min(tr, n_rows - 1), tok = row / p.group;
+        const uint32_t tok = div_group(p, row0 + min(tr, n_rows - 1));
         // positions stay below 2^31
-        const int32_t hi = live ? (int32_t)sp.pos(tok) : -1;
+        const int32_t hi = live ? sp.pos(tok) : -1;
         const int32_t lo = p.window > 0 ? max(hi - (int32_t)p.window + 1, 0) : 0;
         // keys that every live row of the tile attends: blocks inside need no mask
         int32_t all_hi = -1, all_lo = 0;
         if (t < n_tiles) {
-            const int32_t last = (int32_t)sp.pos((min(row0 + n_rows, row0 + 128 * t + 128) - 1) / p.group);
-            all_hi = (int32_t)sp.pos((row0 + 128 * t) / p.group);
+            const int32_t last = sp.pos(div_group(p, min(row0 + n_rows, row0 + 128 * t + 128) - 1));
+            all_hi = sp.pos(div_group(p, row0 + 128 * t));
             all_lo = p.window > 0 ? max(last - (int32_t)p.window + 1, 0) : 0;
         }
         float unscale = 1.0f;
@@ -418,10 +423,11 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
 #pragma unroll
             for (int i = 0; i < HDP / 2; i++) o[i] = 0.0f;
         }
+        // After a wait that ran out (the result is void) the warps go on without waiting, so that no
+        // barrier among them lacks one.
         bool ok = true;
         for (int32_t j = jb[t]; j < je[t]; j++) {
-            ok = mbar_wait_spin(&sm.s_full[t], (j - jb[t]) & 1, p.b.err, ERR_TIMEOUT_FULL);
-            if (!ok) break;
+            ok = ok && mbar_wait_spin(&sm.s_full[t], (j - jb[t]) & 1, p.b.err, ERR_TIMEOUT_FULL);
             tc_fence_after();
             const int32_t key0 = j * kTlBlk + 64 * (int32_t)h;
             const bool part = key0 < all_lo || key0 + 63 > all_hi;
@@ -470,12 +476,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             if constexpr (kSplit) {
                 if (j > jb[t]) {  // add the last block's P V
 #pragma unroll
-                    for (int c = 0; c < HDP / 32; c++) {
-                        uint32_t v[16];
-                        tmem_ld16(to + 16 * c, v);
+                    for (int c = 0; c < HDP / 16; c++) {
+                        uint32_t v[8];
+                        tl_tmem_ld8(to + 8 * c, v);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[16 * c + i] += __uint_as_float(v[i]);
+                        for (int i = 0; i < 8; i++) o[8 * c + i] += __uint_as_float(v[i]);
                     }
                 }
             }
@@ -489,13 +495,13 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                     for (int i = 0; i < HDP / 2; i++) o[i] *= a;
                 } else if (j > jb[t]) {  // the S that was waited for comes after the last P V
 #pragma unroll
-                    for (int c = 0; c < HDP / 32; c++) {
-                        uint32_t v[16];
-                        tmem_ld16(to + 16 * c, v);
+                    for (int c = 0; c < HDP / 16; c++) {  // few registers at a time: the scores hold most
+                        uint32_t v[8];
+                        tl_tmem_ld8(to + 8 * c, v);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-                        tl_tmem_st16(to + 16 * c, v);
+                        for (int i = 0; i < 8; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
+                        tl_tmem_st8(to + 8 * c, v);
                     }
                     tmem_wait_st();
                     tc_fence_before();
@@ -541,7 +547,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         }
         // this tile's MMAs have ended (when a cluster joins, every MMA: O goes over Q and the ring)
         const bool own = je[t] > jb[t];
-        if (p.splits > 1 || own) ok = mbar_wait_spin(p.splits > 1 ? &sm.done : &sm.o_done[t], 0, p.b.err, ERR_TIMEOUT_DRAIN) && ok;
+        if (p.splits > 1 || own) ok = ok && mbar_wait_spin(p.splits > 1 ? &sm.done : &sm.o_done[t], 0, p.b.err, ERR_TIMEOUT_DRAIN);
         tc_fence_after();
         const bool any = own && ok;
         if (t < n_tiles) {
@@ -551,17 +557,17 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             named_bar_sync(pair, 64);
             l = sm.mx[1][tr];
         }
-        // this thread's half of O's columns, 16 at a time
-        auto columns = [&](int c, float (&x)[16]) {
-            uint32_t v[16];
+        // this thread's half of O's columns, 8 at a time
+        auto columns = [&](int c, float (&x)[8]) {
+            uint32_t v[8];
             if (any) {
-                tmem_ld16(to + 16 * c, v);
+                tl_tmem_ld8(to + 8 * c, v);
                 tmem_wait_ld();
             }
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
+            for (int i = 0; i < 8; i++) {
                 x[i] = any ? __uint_as_float(v[i]) : 0.0f;
-                if constexpr (kSplit) x[i] += o[16 * c + i];
+                if constexpr (kSplit) x[i] += o[8 * c + i];
             }
         };
         if (p.splits == 1) {
@@ -572,21 +578,21 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 constexpr int kRowB = HDP * sizeof(T), kVec = kRowB / 16, kPer = 16 / sizeof(T);  // bytes, chunks, values a chunk
                 uint8_t *st = sm.data + t * 128 * kRowB;
                 const float inv = 1.0f / l;
-                bool fine = true;
+                float chk = 0.0f;
 #pragma unroll
-                for (int c = 0; c < HDP / 32; c++) {
-                    float x[16];
+                for (int c = 0; c < HDP / 16; c++) {
+                    float x[8];
                     columns(c, x);
-                    alignas(16) T y[16];
+                    alignas(16) T y[8];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
+                    for (int i = 0; i < 8; i++) {
                         const float f = x[i] * inv;
-                        fine = fine && isfinite(f);
+                        chk = fmaf(f, 0.0f, chk);  // NaN from a value that is not finite
                         y[i] = from_f32<T>(f);
                     }
 #pragma unroll
-                    for (int i = 0; i < (int)sizeof(T); i++)
-                        *reinterpret_cast<uint4 *>(st + r * kRowB + ((((kVec / 2 * h) + (int)sizeof(T) * c + i) ^ (r & 7)) << 4)) =
+                    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+                        *reinterpret_cast<uint4 *>(st + r * kRowB + ((((kVec / 2 * h) + (int)sizeof(T) / 2 * c + i) ^ (r & 7)) << 4)) =
                             reinterpret_cast<const uint4 *>(y)[i];
                 }
                 tc_fence_before();
@@ -598,17 +604,18 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                     const uint32_t i = ((warp & 7) * (16 / kRows) + k) * kRows + lane / kLanes;
                     if (128 * t + i >= n_rows || ch * kPer >= p.hd) continue;
                     const uint32_t rr = row0 + 128 * t + i;
-                    T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + rr / p.group) * p.ld_out +
-                              (uint64_t)(kvh * p.group + rr % p.group) * p.hd;
+                    const uint32_t tk = div_group(p, rr);
+                    T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + tk) * p.ld_out +
+                              (uint64_t)(kvh * p.group + rr - tk * p.group) * p.hd;
                     *reinterpret_cast<uint4 *>(orow + ch * kPer) = *reinterpret_cast<const uint4 *>(st + i * kRowB + ((ch ^ (i & 7)) << 4));
                 }
-                uint32_t bad = __ballot_sync(0xffffffffu, live && !fine);
+                uint32_t bad = __ballot_sync(0xffffffffu, live && chk != 0.0f);
                 named_bar_sync(9 + t, 256);  // every row is written: now the ones that are not finite again
                 while (bad) {
                     const int b = __ffs((int)bad) - 1;
                     bad &= bad - 1;
                     const uint32_t rr = row0 + 128 * t + 32 * (warp & 3) + b;
-                    seq_attn_row<T, E>(p, sp, rr / p.group, kvh, rr % p.group);
+                    seq_attn_row<T, E>(p, sp, div_group(p, rr), kvh, rr - div_group(p, rr) * p.group);
                 }
             }
             tc_fence_before();
@@ -620,12 +627,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         if (t < n_tiles) {
             float *orow = reinterpret_cast<float *>(sm.data) + tr * HDP;
 #pragma unroll
-            for (int c = 0; c < HDP / 32; c++) {
-                float x[16];
+            for (int c = 0; c < HDP / 16; c++) {
+                float x[8];
                 columns(c, x);
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<float4 *>(orow + (((HDP / 8 * h + 4 * c + i) ^ (r & (HDP / 4 - 1))) << 2)) =
+                for (int i = 0; i < 2; i++)
+                    *reinterpret_cast<float4 *>(orow + (((HDP / 8 * h + 2 * c + i) ^ (r & (HDP / 4 - 1))) << 2)) =
                         make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
         }
@@ -668,7 +675,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 const float4 x = ld_cluster_f32x4(cluster_addr(a, c));
                 if (w != 0.0f) v = make_float4(fmaf(w, x.x, v.x), fmaf(w, x.y, v.y), fmaf(w, x.z, v.z), fmaf(w, x.w, v.w));
             }
-            const uint32_t rr = row0 + (in ? i : 0), tk = rr / p.group, gq = rr % p.group;
+            const uint32_t rr = row0 + (in ? i : 0), tk = div_group(p, rr), gq = rr - tk * p.group;
             T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + tk) * p.ld_out + (uint64_t)(kvh * p.group + gq) * p.hd;
             const bool fine = !in || 4 * ch >= p.hd || (isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
             if (in && 4 * ch < p.hd) {
@@ -682,7 +689,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 for (int k = 0; k < 32 / kVec; k++)
                     if (bad >> (k * kVec) & (kVec == 32 ? 0xffffffffu : (1u << kVec) - 1)) {
                         const uint32_t rb = __shfl_sync(0xffffffffu, rr, k * kVec);
-                        seq_attn_row<T, E>(p, sp, rb / p.group, kvh, rb % p.group);
+                        seq_attn_row<T, E>(p, sp, div_group(p, rb), kvh, rb - div_group(p, rb) * p.group);
                     }
             }
         }

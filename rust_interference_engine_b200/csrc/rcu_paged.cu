@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) k_paged_store(const SeqView b, const T *_
     uint32_t first;
     const uint32_t n = seq_rows(b, seq, &first);
     if (t < first || t - first >= n) return;  // offsets out of order (reported)
-    const int64_t pos = seq_len(b, seq, n) - (int64_t)n + (int64_t)(t - first);
+    const int32_t pos = seq_len(b, seq, n) - (int32_t)n + (int32_t)(t - first);
     if (pos < 0) return;  // a length shorter than the new tokens (reported)
     const uint32_t pg = seq_page(b, seq, (uint32_t)(pos >> b.page_shift));
     if (pg == kNoRow) return;
@@ -243,7 +243,7 @@ int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s
     p.kv_rows = (uint32_t)(pg->n_pages * pg->n_kv * pg->page_size);
     p.n_head = (uint32_t)n_head;
     p.n_kv = (uint32_t)pg->n_kv;
-    p.group = (uint32_t)(n_head / pg->n_kv);
+    set_group(p, (uint32_t)(n_head / pg->n_kv));
     p.hd = (uint32_t)pg->hd;
     p.window = (uint32_t)window;
     p.softcap = softcap;
@@ -282,7 +282,7 @@ int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, u
     p.kv_rows = (uint32_t)n_tok;
     p.n_head = (uint32_t)n_head;
     p.n_kv = (uint32_t)n_head_kv;
-    p.group = (uint32_t)(n_head / n_head_kv);
+    set_group(p, (uint32_t)(n_head / n_head_kv));
     p.hd = (uint32_t)head_dim;
     p.window = (uint32_t)window;
     p.softcap = softcap;

@@ -30,9 +30,9 @@ struct SeqView {
 // What one sequence of the batch is, clamped to the batch and to its page table.
 struct SeqSpan {
     uint32_t seq, first, n_new;  // rows first .. first + n_new - 1
-    int64_t len;                 // positions 0 .. len - 1 are in the cache
+    int32_t len;                 // positions 0 .. len - 1 are in the cache (the host keeps tables below 2^31)
     // position of new token t: negative where a wrong len is shorter than n_new (no keys then)
-    __device__ __forceinline__ int64_t pos(uint32_t t) const { return len - (int64_t)n_new + (int64_t)t; }
+    __device__ __forceinline__ int32_t pos(uint32_t t) const { return len - (int32_t)n_new + (int32_t)t; }
 };
 
 __device__ __forceinline__ uint32_t seq_rows(const SeqView &b, uint32_t s, uint32_t *first) {
@@ -42,11 +42,11 @@ __device__ __forceinline__ uint32_t seq_rows(const SeqView &b, uint32_t s, uint3
     *first = (uint32_t)a0;
     return (uint32_t)(a1 - a0);
 }
-__device__ __forceinline__ int64_t seq_len(const SeqView &b, uint32_t s, uint32_t n_new) {
-    if (!b.len) return n_new;
-    const int64_t cap = (int64_t)b.ld_pages << b.page_shift, l = b.len[s];
-    if (l < (int64_t)n_new || l > cap) atomicOr(b.err, (uint32_t)ERR_BAD_ARG);
-    return min(max(l, (int64_t)0), cap);
+__device__ __forceinline__ int32_t seq_len(const SeqView &b, uint32_t s, uint32_t n_new) {
+    if (!b.len) return (int32_t)n_new;
+    const int32_t cap = (int32_t)(b.ld_pages << b.page_shift), l = b.len[s];  // the host keeps cap below 2^31
+    if (l < (int32_t)n_new || l > cap) atomicOr(b.err, (uint32_t)ERR_BAD_ARG);
+    return min(max(l, 0), cap);
 }
 
 // The sequence that holds work tile `ti` when each sequence takes ceil(n_new * group / rows) tiles,
@@ -103,6 +103,12 @@ __device__ __forceinline__ uint32_t seq_kv_row(const SeqView &b, const SeqSpan &
     const uint32_t pg = seq_page(b, sp.seq, pos >> b.page_shift);
     if (pg == kNoRow) return kNoRow;
     return ((pg * n_kv + kvh) << b.page_shift) + (pos & ((1u << b.page_shift) - 1));
+}
+
+// x, of which the compiler knows nothing: what is computed from it is not kept from before.
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
 }
 
 // ---- elements ---------------------------------------------------------------------------------
@@ -234,8 +240,23 @@ struct SeqAttnParams {
     uint64_t ld_kv, head_kv;    // elements between rows of k / v, and between a row's kv heads
     uint32_t kv_rows;           // rows of k / v
     uint32_t n_head, n_kv, group, hd, window, n_tiles, splits;
+    uint64_t group_mul;         // n / group = n * group_mul >> group_shift for n < 2^31
+    uint32_t group_shift;
     float softcap;
 };
+
+// n < 2^31 divided by the group: with 2^s >= group, group_mul = floor(2^(31 + s) / group) + 1 is off by
+// at most one part in 2^(31 + s) / group, which n < 2^31 cannot carry to the next whole number.
+__device__ __forceinline__ uint32_t div_group(const SeqAttnParams &p, uint32_t n) {
+    return (uint32_t)((uint64_t)n * p.group_mul >> p.group_shift);
+}
+inline void set_group(SeqAttnParams &p, uint32_t group) {
+    uint32_t s = 0;
+    while ((1u << s) < group) s++;
+    p.group = group;
+    p.group_shift = 31 + s;
+    p.group_mul = (1ull << (31 + s)) / group + 1;
+}
 
 // One output row by one warp, from the formula, over the attended keys alone. The tiled kernels
 // multiply the probability 0 of a masked key with its value, which is NaN where that value is an
@@ -244,8 +265,7 @@ struct SeqAttnParams {
 template <typename T, typename E>
 __device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan &sp, uint32_t t, uint32_t kvh, uint32_t g) {
     const uint32_t lane = threadIdx.x & 31, head = kvh * p.group + g;
-    const int64_t pos = sp.pos(t);
-    const int64_t lo = p.window > 0 && pos + 1 > (int64_t)p.window ? pos + 1 - p.window : 0;
+    const int32_t pos = sp.pos(t), lo = p.window > 0 ? max(pos - (int32_t)p.window + 1, 0) : 0;
     const T *q = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + t) * p.ld_q + (uint64_t)head * p.hd;
     T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + t) * p.ld_out + (uint64_t)head * p.hd;
     const uint32_t kvo = p.b.pages ? 0u : kvh * (uint32_t)p.head_kv;
@@ -257,7 +277,7 @@ __device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan 
         o[i] = 0.0f;
     }
     float m = -INFINITY, l = 0.0f;
-    for (int64_t j = lo; j <= pos; j++) {
+    for (int64_t j = lo; j <= pos; j++) {  // pos may be 2^31 - 1
         const uint32_t row = seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)j);
         const E *kr = reinterpret_cast<const E *>(p.k) + (uint64_t)row * p.ld_kv + kvo;
         const E *vr = reinterpret_cast<const E *>(p.v) + (uint64_t)row * p.ld_kv + kvo;
