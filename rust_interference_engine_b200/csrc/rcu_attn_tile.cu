@@ -22,6 +22,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "rcu_kernels.h"
@@ -713,8 +714,18 @@ static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64
     constexpr size_t smem = sizeof(TlSmem<HDP, std::is_same<T, float>::value>);
     static_assert(smem <= 232448, "shared memory of one CTA");
     const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + kTlRows) : max_len;
-    uint32_t cs = 1;  // one CTA for each SM, four blocks of keys for each
-    while (cs < kTlMaxCluster && items * cs * 2 <= (uint64_t)ctx->num_sms && span >= (uint64_t)cs * 2 * 4 * kTlBlk) cs *= 2;
+    // CTAs per tile by the time they take, in blocks of keys: each its share and, for its start, its end
+    // and the join, about 5 (alone) or 7 more; the last wave is half full on average. Sequences of
+    // different lengths count as 0.6 of the longest. (16 sequences of 250 .. 5000 keys, two chunks among
+    // them: 79 us alone, 64 us by two, 88 us by four; one chunk over 12,800 keys: 177 us by two, 186 by four.)
+    const double blocks = (double)((span + kTlBlk - 1) / kTlBlk);
+    uint32_t cs = 1;
+    double best = 0.0;
+    for (uint32_t c = 1; c <= kTlMaxCluster && (c == 1 || blocks >= 2.0 * c); c *= 2) {
+        const double f = (double)items * c / ctx->num_sms, waves = f <= 1.0 ? 1.0 : p.b.n_seq > 1 ? 0.6 * f + 0.5 : std::ceil(f);
+        const double cost = waves * (blocks / c + (c == 1 ? 5.0 : 7.0));
+        if (c == 1 || cost < best) best = cost, cs = c;
+    }
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
     return launch_cluster_k<k_attn_tile<T, E, HDP>>(ctx, (uint32_t)(items * cs), kTlThreads, smem, cs, m.k, m.v, p);
