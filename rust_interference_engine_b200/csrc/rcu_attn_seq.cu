@@ -423,11 +423,12 @@ template <typename T, typename E, int HDP, int NT>
 static int launch_few(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64_t max_len) {
     const size_t smem = sizeof(SqSmem<HDP>) + 1024;
     p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, (std::is_same<T, float>::value ? 4 : 8) * NT);
-    // CTAs per tile: up to three for each SM in all, and at least 128 keys each
+    // CTAs per tile: up to three for each SM in all, and at least 64 keys each (a chunk for each warp;
+    // eight warps a CTA instead were slower: clusters of 16 such CTAs do not all find SMs at once)
     const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + 16) : max_len;
     const uint32_t most = HDP == 256 ? 8 : kSqMaxCluster;  // one CTA to an SM: eight SMs of a GPC are sure to be there
     uint32_t cs = 1;
-    while (cs < most && items * cs * 2 <= 3ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 128) cs *= 2;
+    while (cs < most && items * cs * 2 <= 3ull * ctx->num_sms && span >= (uint64_t)cs * 2 * 64) cs *= 2;
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
     return launch_cluster_k<k_attn_seq<T, E, HDP, NT>>(ctx, (uint32_t)(items * cs), kSqWarps * 32, smem, cs, m.k, m.v, p);

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) k_paged_store(const SeqView b, const T *_
     uint32_t first;
     const uint32_t n = seq_rows(b, seq, &first);
     if (t < first || t - first >= n) return;  // offsets out of order (reported)
-    const int32_t pos = seq_len(b, seq, n) - (int32_t)n + (int32_t)(t - first);
+    const int32_t pos = seq_len(b, b.len[seq], n) - (int32_t)n + (int32_t)(t - first);
     if (pos < 0) return;  // a length shorter than the new tokens (reported)
     const uint32_t pg = seq_page(b, seq, (uint32_t)(pos >> b.page_shift));
     if (pg == kNoRow) return;

@@ -42,9 +42,10 @@ __device__ __forceinline__ uint32_t seq_rows(const SeqView &b, uint32_t s, uint3
     *first = (uint32_t)a0;
     return (uint32_t)(a1 - a0);
 }
-__device__ __forceinline__ int32_t seq_len(const SeqView &b, uint32_t s, uint32_t n_new) {
+// The length l that the batch gives for a sequence of n_new new tokens, clamped to its table.
+__device__ __forceinline__ int32_t seq_len(const SeqView &b, int32_t l, uint32_t n_new) {
     if (!b.len) return (int32_t)n_new;
-    const int32_t cap = (int32_t)(b.ld_pages << b.page_shift), l = b.len[s];  // the host keeps cap below 2^31
+    const int32_t cap = (int32_t)(b.ld_pages << b.page_shift);  // the host keeps it below 2^31
     if (l < (int32_t)n_new || l > cap) atomicOr(b.err, (uint32_t)ERR_BAD_ARG);
     return min(max(l, 0), cap);
 }
@@ -58,7 +59,12 @@ __device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, 
     uint32_t base = 0;
     for (uint32_t s0 = 0; s0 < b.n_seq; s0 += 32) {
         uint32_t first = 0, n = 0;
-        if (s0 + lane < b.n_seq) n = seq_rows(b, s0 + lane, &first);
+        int32_t len = 0;
+        if (s0 + lane < b.n_seq) {
+            const int32_t l = b.len ? b.len[s0 + lane] : 0;  // on its way together with the offsets
+            n = seq_rows(b, s0 + lane, &first);
+            len = seq_len(b, l, n);
+        }
         const uint32_t t = (n * group + rows - 1) / rows;  // below 2^31: the host checks n_tok * group
         uint32_t inc = t;
 #pragma unroll
@@ -73,7 +79,7 @@ __device__ __forceinline__ bool seq_find_tile(const SeqView &b, uint32_t group, 
             sp->first = __shfl_sync(0xffffffffu, first, l);
             sp->n_new = __shfl_sync(0xffffffffu, n, l);
             *tile = ti - base - (__shfl_sync(0xffffffffu, inc, l) - __shfl_sync(0xffffffffu, t, l));
-            sp->len = seq_len(b, sp->seq, sp->n_new);
+            sp->len = __shfl_sync(0xffffffffu, len, l);
             return true;
         }
         base += __shfl_sync(0xffffffffu, inc, 31);
