@@ -444,6 +444,7 @@ class SeqBatch:
         for x, what, dims in ((cu, "cu", 1), (len, "len", 1), (pages, "pages", 2)):
             if str(x.dtype) != "torch.int32" or x.dim() != dims or not x.is_contiguous():
                 raise ValueError(f"{what}: expected a contiguous {dims}-dimensional int32 tensor")
+        for x, what in ((cu, "cu"), (len, "len"), (pages, "pages")):
             if not x.is_cuda or x.get_device() != cu.get_device():
                 raise ValueError(f"{what}: expected a CUDA tensor on the batch's device")
         n_seq = len.shape[0]

@@ -355,3 +355,100 @@ def test_calls_on_two_streams_do_not_share_anything(env):
         c.check(o[0])
         for x in o[1:]:
             assert torch.equal(x, o[0])  # the same bits every time
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16"])
+@pytest.mark.parametrize("hd", [160, 224])
+def test_head_dims_between(env, ty, hd):
+    c = Case(*env, [(1, 70), (9, 33), (40, 80)], 4, 2, hd, 16, ty, seed=20)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("new", [1, 2])
+def test_hundreds_of_sequences(env, new):
+    """The lookup of a tile's sequence goes over many groups of 32, empty sequences among them."""
+    seqs = [(new if i % 7 else 0, 3 + (i * 37) % 90) for i in range(333)]
+    c = Case(*env, seqs, 4, 2, 64, 16, "f16", seed=21)
+    c.check(c.run())
+    c.check(c.run(max_len=100))
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16"])
+@pytest.mark.parametrize("window", [0, 300, 1500])
+def test_chunk_split_over_a_cluster(env, ty, window):
+    """A chunk late in a long context: its keys are split, windows leave some parts without any."""
+    c = Case(*env, [(70, 6000)], 4, 1, 128, 64, ty, seed=22)
+    c.check(c.run(window), window)
+    c.check(c.run(window, 25.0), window, 25.0)
+
+
+@pytest.mark.parametrize("max_new", [0, 1, 12, 500])
+def test_max_new_shapes_the_launch_only(env, max_new):
+    """A wrong max_new chooses another kernel, with the same result."""
+    torch, rie, ctx = env
+    c = Case(torch, rie, ctx, [(12, 90), (1, 400), (500, 500), (3, 17)], 8, 2, 128, 32, "f16", seed=23)
+    out = torch.full_like(c.q, 7.5)
+    rie.paged_attention(ctx, c.cache, rie.SeqBatch(*c.dev, c.n_tok, max_new=max_new), c.q, 8, out)
+    ctx.sync()
+    c.check(out)
+
+
+@pytest.mark.parametrize("n", [17, 300])
+def test_nan_and_infinite_queries(env, n):
+    """A query that is not finite makes its own row NaN, and no other."""
+    torch, rie, ctx = env
+    for ty in ("f32", "f16"):
+        c = Case(torch, rie, ctx, [(n, n + 20)], 4, 2, 128, 16, ty, seed=24)
+        want = c.run()
+        c.q[3, 128 + 5] = float("nan")
+        c.q[7, 5] = float("inf")
+        out = c.run()
+        bad = torch.zeros(c.n_tok, 4, dtype=torch.bool)
+        bad[3, 1] = bad[7, 0] = True
+        rows = out.view(c.n_tok, 4, 128).cpu()
+        assert torch.isnan(rows[bad]).all()
+        assert torch.equal(rows[~bad], want.view(c.n_tok, 4, 128).cpu()[~bad])
+
+
+def test_pages_shared_by_two_sequences(env):
+    """A common prefix in the same pages, and the same page twice in a table."""
+    torch, rie, ctx = env
+    c = Case(torch, rie, ctx, [(1, 64), (1, 64)], 4, 2, 64, 16, "f16", seed=25)
+    c.dev[2][1, :3] = c.dev[2][0, :3]
+    c.dev[2][1, 1] = c.dev[2][0, 0]
+    for x in (c.ks, c.vs):
+        x[1][:48] = x[0][:48]
+        x[1][16:32] = x[0][:16]
+    c.check(c.run())
+
+
+def test_owned_pool_starts_zeroed_and_serves(env):
+    """Pages of the library's own; append, then attention, step by step next to one LayerCache a
+    sequence: two f32 attentions over the same f16 rows."""
+    torch, rie, ctx = env
+    n_head, n_kv, hd, ps, n_pages = 8, 2, 128, 16, 40
+    cache = rie.PagedCache(ctx, n_kv, hd, ps, n_pages)
+    k_ptr, v_ptr = cache.data_ptrs()
+    assert k_ptr and v_ptr and k_ptr != v_ptr
+    lens = [0, 0, 0]
+    flat = [rie.LayerCache(ctx, rie.KvType.F16, n_kv, hd, 256) for _ in lens]
+    pages = torch.arange(30, dtype=torch.int32, device="cuda").reshape(10, 3).t().contiguous()
+    g = torch.Generator(device="cuda").manual_seed(26)
+    for new in ([50, 3, 17], [1, 1, 1], [1, 0, 1], [20, 1, 2], [1, 1, 1]):
+        n = sum(new)
+        cu = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32, device="cuda")
+        lens = [a + b for a, b in zip(lens, new)]
+        batch = rie.SeqBatch(cu, torch.tensor(lens, dtype=torch.int32, device="cuda"), pages, n, max_len=max(lens))
+        q, k, v = (torch.randn(n, h * hd, generator=g, device="cuda") * s for h, s in ((n_head, hd ** -0.5), (n_kv, 1), (n_kv, 1)))
+        out, want = torch.zeros_like(q), torch.zeros_like(q)
+        cache.store(batch, k, v)
+        rie.paged_attention(ctx, cache, batch, q, n_head, out)
+        at = 0
+        for c, length, m in zip(flat, lens, new):
+            if m:
+                c.store(k[at:at + m], v[at:at + m], m, length - m)
+                rie.attention(ctx, c, q[at:at + m], m, n_head, length - m, want[at:at + m])
+            at += m
+        ctx.sync()
+        # both are the same sums in f32, in another order: 2^-20 of values below 4 (the split parts carry 2^-22)
+        assert (out - want).abs().max().item() <= 4 * 2.0 ** -18
