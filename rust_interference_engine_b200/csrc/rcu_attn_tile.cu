@@ -2,12 +2,13 @@
 // whole prompts) on the 5th-generation tensor cores. Formula and batch as in rcu_attn_seq.cu.
 //
 // A CTA takes 256 query rows (token, head of the group) of one sequence and KV head as two tiles of
-// 128 rows, and walks the attended keys in blocks of 128:
+// 128 rows (head_dim above 128: one tile, since O fills tensor memory), and walks the attended keys in
+// blocks of 128:
 //   * warp 16    producer: K and V blocks by tiled TMA (128-byte swizzle) into a ring of stages; a
 //                page may be smaller than a block (one box per page) or larger;
 //   * warp 17    owns tensor memory; one thread issues S_t = Q_t K^T (M 128, N 128) and O_t += P_t V
 //                (P read from tensor memory, V in its own layout as an MN-major operand);
-//   * warps 0-15 softmax, 8 for each tile: two threads share a query row, one for the first 64 keys of
+//   * warps 0-15 softmax, 8 for each tile (one tile: warps 0-7, and 8 and 9 for the above): two threads share a query row, one for the first 64 keys of
 //                the block and one for the others: S out of tensor memory, mask, running maximum
 //                (the two exchange theirs) and sum in f32, P = 2^(s - m) back as packed 16-bit values
 //                over S, each half handed on by itself.
@@ -31,31 +32,33 @@
 
 namespace rcu {
 
-constexpr int kTlRows = 256;       // query rows per CTA (two tiles)
 constexpr int kTlBlk = kSeqTileBox;  // keys per block
-constexpr int kTlSoftWarps = 16;
-constexpr int kTlThreads = 640;    // four softmax warpgroups; a fifth for the producer and the MMA issuer
-// registers a thread: the fifth warpgroup gives its own up (4 x 112 + 32 = 5 x 96, the launch's)
-constexpr int kTlRegsSoftmax = 112, kTlRegsOther = 32;
 constexpr int kTlMaxCluster = 8;
-constexpr int kTlPoly = 2;         // of 8 exponential pairs: on the FMA pipe, beside the special-function unit
 constexpr float kTlLazy = 8.0f, kTlShift = 7.0f;
 
 template <int HDP, bool SPLIT>
 struct TlCfg {
+    static constexpr int kTiles = HDP == 256 ? 1 : 2;
+    static constexpr int kRows = 128 * kTiles;               // query rows per CTA
+    static constexpr int kSoftWarps = 8 * kTiles;
+    static constexpr int kThreads = 32 * (kSoftWarps + 4);   // a warpgroup for the producer and the MMA issuer
+    // registers a thread: the last warpgroup gives its own up (4 x 112 + 32 = 5 x 96, or 2 x 224 + 56 =
+    // 3 x 168, the launch's)
+    static constexpr int kRegsSoftmax = kTiles == 2 ? 112 : 224, kRegsOther = kTiles == 2 ? 32 : 56;
     static constexpr int kPart = 128 * HDP * 2;              // one tile's Q (one part of it)
     static constexpr int kParts = SPLIT ? 2 : 1;
-    static constexpr int kQ = 2 * kParts * kPart;
+    static constexpr int kQ = kTiles * kParts * kPart;
     static constexpr int kStage = kTlBlk * HDP * 2;          // one K or V block
-    static constexpr int kStages = HDP == 64 ? 8 : SPLIT ? 3 : 5;
+    static constexpr int kStages = HDP == 64 ? 8 : HDP == 256 ? 2 : SPLIT ? 3 : 5;
     static constexpr int kData = kQ + kStages * kStage;
-    static_assert(kData >= kTlRows * HDP * 4 + 8 * kTlRows * 4, "the joined O and its weights overlay Q and the ring");
+    static_assert(kData >= kRows * HDP * 4 + kTlMaxCluster * kRows * 4, "the joined O and its weights overlay Q and the ring");
+    static_assert(!(SPLIT && HDP == 256), "Q's two parts leave no room for a ring");
 };
 template <int HDP, bool SPLIT>
 struct TlSmem {
     using C = TlCfg<HDP, SPLIT>;
     uint8_t data[C::kData];  // Q, then the ring; at the end O and its weights when a cluster joins
-    float mx[2][kTlRows];    // [half of the block's keys]: row maxima; at the end the row's m and l
+    float mx[2][C::kRows];   // [half of the block's keys]: row maxima; at the end the row's m and l
     uint64_t full[C::kStages], empty[C::kStages], s_full[2], p_half[2], p_full[2], o_done[2], done;
     uint32_t tmem;
 };
@@ -116,25 +119,6 @@ __device__ __forceinline__ float tl_max16(const uint32_t (&s)[16]) {
         c[i] = max3_nan(__uint_as_float(s[3 * i]), __uint_as_float(s[3 * i + 1]), __uint_as_float(s[3 * i + 2]));
     return max3_nan(max3_nan(c[0], c[1], c[2]), max3_nan(c[3], c[4], __uint_as_float(s[15])), -INFINITY);
 }
-// 2^x of two values on the FMA pipe, x <= 127 (below -126: 2^-126): x = n + f with n the nearest
-// whole number (from the addition of 1.5 * 2^23), 2^f by the polynomial of least relative error on
-// [-1/2, 1/2] (degree 4: 2.6e-6, degree 3: 7.5e-5; exchange algorithm in 64 bits), n into the exponent.
-template <int DEG>
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
-    const float2 t = add2(x, make_float2(12582912.0f, 12582912.0f));
-    const float2 n = add2(t, make_float2(-12582912.0f, -12582912.0f));
-    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-    constexpr float c[2][5] = {{0.9999280571937561f, 0.6932609677314758f, 0.2426111251115799f, 0.0551716685295105f, 0.0f},
-                               {0.9999992847442627f, 0.6931217908859253f, 0.240247443318367f, 0.05591785907745361f, 0.009570102207362652f}};
-    float2 y = make_float2(c[DEG - 3][DEG], c[DEG - 3][DEG]);
-#pragma unroll
-    for (int i = DEG - 1; i >= 0; i--) y = fma2(y, f, make_float2(c[DEG - 3][i], c[DEG - 3][i]));
-    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23));
-    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23));
-    return y;
-}
-
 // Blocks [lo, hi) of keys that rows [r0, r1) of a sequence attend (r1 > r0).
 struct TlSpan {
     int32_t lo, hi;
@@ -146,13 +130,13 @@ __device__ __forceinline__ TlSpan tl_span(const SeqAttnParams &p, const SeqSpan 
 }
 
 template <typename T, typename E, int HDP>
-__global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kThreads, 1) k_attn_tile(const __grid_constant__ CUtensorMap mk,
                                                              const __grid_constant__ CUtensorMap mv,
                                                              const __grid_constant__ SeqAttnParams p) {
     constexpr bool kSplit = std::is_same<T, float>::value;
     using C = TlCfg<HDP, kSplit>;
     using S = TlSmem<HDP, kSplit>;
-    constexpr int kChunks = HDP / 64;
+    constexpr int kChunks = HDP / 64, kTiles = C::kTiles, kTlRows = C::kRows, kTlSoftWarps = C::kSoftWarps;
     extern __shared__ __align__(1024) uint8_t tl_raw[];  // swizzled tiles start on 1024-byte boundaries
     S &sm = *reinterpret_cast<S *>(tl_raw);
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -163,7 +147,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
     if (warp == kTlSoftWarps) {
         if (lane == 0) {
             for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < kTiles; t++)
                 mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_half[t], 4), mbar_init(&sm.p_full[t], 4), mbar_init(&sm.o_done[t], 1);
             mbar_init(&sm.done, 1);
             fence_mbar_init();
@@ -179,14 +163,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
         return;
     }
     const uint32_t row0 = tile * kTlRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kTlRows);
-    const uint32_t n_tiles = n_rows > 128 ? 2 : 1;
+    const uint32_t n_tiles = n_rows > 128 ? 2 : 1;  // 1 where there is one
     // this CTA's part of the blocks, and each tile's part of those
     const TlSpan all = tl_span(p, sp, row0, row0 + n_rows);
     const int32_t per = (all.hi - all.lo + (int32_t)p.splits - 1) / (int32_t)p.splits;
     const int32_t j0 = min(all.lo + (int32_t)rank * per, all.hi), j1 = min(j0 + per, all.hi);
-    int32_t jb[2], je[2];
+    int32_t jb[2] = {j0, j0}, je[2] = {j0, j0};
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
+    for (int t = 0; t < kTiles; t++) {
         jb[t] = je[t] = j0;
         if (t < (int)n_tiles) {
             const TlSpan s = tl_span(p, sp, row0 + 128 * t, min(row0 + n_rows, row0 + 128 * t + 128));
@@ -268,7 +252,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
     };
     if (warp != kTlSoftWarps) meet();  // the producer has its copies on their way first
     if (warp >= kTlSoftWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTlRegsOther));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
     }
     if (warp == kTlSoftWarps) {  // ---- producer ----
         bool met = false;
@@ -338,8 +322,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             }
             if (!last) wait(&sm.full[sk], pk);
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t ts = tm + 128 * t, to = tm + 256 + HDP * t;
+            for (int t = 0; t < kTiles; t++) {
+                const uint32_t ts = tm + 128 * t, to = tm + 128 * kTiles + HDP * t;
                 const int32_t b = t ? b1 : b0, e = t ? e1 : e0;
                 if (j - 1 >= b && j - 1 < e && ok) {  // O_t += P_t V(j - 1)
                     const uint64_t v = dv + sv * (C::kStage >> 4);
@@ -358,7 +342,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                     np[t]++;
                     if (j == e && elected) mma_commit(&sm.o_done[t]);
                 }
-                if (t == 1 && j > 0 && elected) mma_commit(&sm.empty[sv]);
+                if (t == kTiles - 1 && j > 0 && elected) mma_commit(&sm.empty[sv]);
                 if (j >= b && j < e && ok) {  // S_t = Q_t K(j)^T
                     if (elected) {
                         const uint64_t k = dk + sk * (C::kStage >> 4), q = dq + t * ((C::kParts * C::kPart) >> 4);
@@ -389,17 +373,18 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             next(sk, pk);
         }
         if (elected) {
-            if (!ok) mma_commit(&sm.o_done[0]), mma_commit(&sm.o_done[1]);
+            if (!ok)
+                for (int t = 0; t < kTiles; t++) mma_commit(&sm.o_done[t]);
             mma_commit(&sm.done);  // every MMA issued, on an early end too
         }
         __syncwarp();
         mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN);
     } else if (warp < kTlSoftWarps) {  // ---- softmax: row r of tile t, keys 64 h .. 64 h + 63 of each block ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTlRegsSoftmax));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
         const uint32_t t = warp >> 3, h = (warp >> 2) & 1, r = threadIdx.x & 127, tr = 128 * t + r;
         const uint32_t pair = 1 + 4 * t + (warp & 3);    // barrier of the two warps that share these rows
         const uint32_t lanes = (32 * (warp & 3)) << 16;  // their TMEM lanes
-        const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 256 + HDP * t + HDP / 2 * h + lanes;
+        const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 128 * kTiles + HDP * t + HDP / 2 * h + lanes;
         const bool live = tr < n_rows;
         const uint32_t tok = div_group(p, row0 + min(tr, n_rows - 1));
         // positions stay below 2^31
@@ -525,9 +510,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
                 for (int i = 0; i < 8; i++) {
                     const float2 y = fma2(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])),
                                           make_float2(cs, cs), make_float2(-off, -off));
-                    float2 e;
-                    if (!kSplit && i < kTlPoly) e = ex2_poly<std::is_same<E, __half>::value ? 4 : 3>(y);
-                    else e = make_float2(ex2(y.x), ex2(y.y));
+                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
                     if (i & 1) sum1 = add2(sum1, e);
                     else sum0 = add2(sum0, e);
                     u[i] = pack2<E>(e.x, e.y);
@@ -544,7 +527,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(h ? &sm.p_full[t] : &sm.p_half[t]);
             l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-            if (mx != mx) l = mx;  // a NaN among the scores (the polynomial does not carry it)
         }
         // this tile's MMAs have ended (when a cluster joins, every MMA: O goes over Q and the ring)
         const bool own = je[t] > jb[t];
@@ -662,24 +644,28 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             if (!isfinite(inv)) wt[i] = __uint_as_float(0x7fffffffu);  // no keys, or a NaN: the row is made again
         }
         named_bar_sync(15, kTlSoftWarps * 32);
-        constexpr int kVec = HDP / 4;  // 16-byte chunks of a row
-        const uint32_t step = p.splits * kTlSoftWarps * 32 / kVec, ch = lane % kVec;
+        constexpr int kVec = HDP / 4, kLn = kVec < 32 ? kVec : 32, kPerRow = kVec / kLn;  // 16-byte chunks of a row, lanes, chunks a lane
+        const uint32_t step = p.splits * kTlSoftWarps * 32 / kLn;
 #pragma unroll 2
-        for (uint32_t i = (rank * kTlSoftWarps + warp) * (32 / kVec) + lane / kVec; i - lane / kVec < n_rows; i += step) {
+        for (uint32_t i = (rank * kTlSoftWarps + warp) * (32 / kLn) + lane / kLn; i - lane / kLn < n_rows; i += step) {
             const bool in = i < n_rows;
-            const uint32_t a = smem_u32(sm.data) + (in ? i * HDP * 4 + ((ch ^ (i & (kVec - 1))) << 4) : 0);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < kTlMaxCluster; c++) {
-                if (c >= (int)p.splits || !in) continue;
-                const float w = wt[c * kTlRows + i];
-                const float4 x = ld_cluster_f32x4(cluster_addr(a, c));
-                if (w != 0.0f) v = make_float4(fmaf(w, x.x, v.x), fmaf(w, x.y, v.y), fmaf(w, x.z, v.z), fmaf(w, x.w, v.w));
-            }
             const uint32_t rr = row0 + (in ? i : 0), tk = div_group(p, rr), gq = rr - tk * p.group;
             T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + tk) * p.ld_out + (uint64_t)(kvh * p.group + gq) * p.hd;
-            const bool fine = !in || 4 * ch >= p.hd || (isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
-            if (in && 4 * ch < p.hd) {
+            bool fine = true;
+#pragma unroll
+            for (int u = 0; u < kPerRow; u++) {
+                const uint32_t ch = lane % kLn + 32 * u;
+                const uint32_t a = smem_u32(sm.data) + (in ? i * HDP * 4 + ((ch ^ (i & (kVec - 1))) << 4) : 0);
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < kTlMaxCluster; c++) {
+                    if (c >= (int)p.splits || !in) continue;
+                    const float w = wt[c * kTlRows + i];
+                    const float4 x = ld_cluster_f32x4(cluster_addr(a, c));
+                    if (w != 0.0f) v = make_float4(fmaf(w, x.x, v.x), fmaf(w, x.y, v.y), fmaf(w, x.z, v.z), fmaf(w, x.w, v.w));
+                }
+                if (!in || 4 * ch >= p.hd) continue;
+                fine = fine && isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(orow + 4 * ch) = v;
                 else *reinterpret_cast<uint2 *>(orow + 4 * ch) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
             }
@@ -687,9 +673,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
             if (bad) {
                 __syncwarp();
 #pragma unroll 1
-                for (int k = 0; k < 32 / kVec; k++)
-                    if (bad >> (k * kVec) & (kVec == 32 ? 0xffffffffu : (1u << kVec) - 1)) {
-                        const uint32_t rb = __shfl_sync(0xffffffffu, rr, k * kVec);
+                for (int r = 0; r < 32 / kLn; r++)
+                    if (bad >> (r * kLn) & (kLn == 32 ? 0xffffffffu : (1u << kLn) - 1)) {
+                        const uint32_t rb = __shfl_sync(0xffffffffu, rr, r * kLn);
                         seq_attn_row<T, E>(p, sp, div_group(p, rb), kvh, rb - div_group(p, rb) * p.group);
                     }
             }
@@ -707,13 +693,15 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile(const __grid_consta
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-bool attention_tile_ok(uint64_t hd) { return hd <= 128; }
+bool attention_tile_ok(uint64_t hd, int q_type) { return hd <= 128 || q_type != T_F32; }
 
 template <typename T, typename E, int HDP>
 static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64_t max_len) {
+    using C = TlCfg<HDP, std::is_same<T, float>::value>;
     constexpr size_t smem = sizeof(TlSmem<HDP, std::is_same<T, float>::value>);
+    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, C::kRows);
     static_assert(smem <= 232448, "shared memory of one CTA");
-    const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + kTlRows) : max_len;
+    const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + C::kRows) : max_len;
     // CTAs per tile by the time they take, in blocks of keys: each its share and, for its start, its end
     // and the join, about 5 (alone) or 7 more; the last wave is half full on average. Sequences of
     // different lengths count as 0.6 of the longest. (16 sequences of 250 .. 5000 keys, two chunks among
@@ -728,7 +716,7 @@ static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64
     }
     p.splits = cs;
     if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
-    return launch_cluster_k<k_attn_tile<T, E, HDP>>(ctx, (uint32_t)(items * cs), kTlThreads, smem, cs, m.k, m.v, p);
+    return launch_cluster_k<k_attn_tile<T, E, HDP>>(ctx, (uint32_t)(items * cs), C::kThreads, smem, cs, m.k, m.v, p);
 }
 
 template <typename T, typename E>
@@ -736,8 +724,10 @@ static int launch_tile_hd(rcu_ctx *ctx, SeqAttnParams &p, const SeqKvDesc &kv, u
     SeqKvMaps room;
     const SeqKvMaps *m;
     if (int st = seq_pick_maps(ctx, p, kv, kSeqTileBox, kv.tile, &room, &m)) return st;
-    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, kTlRows);
-    return p.hd <= 64 ? launch_tile<T, E, 64>(ctx, *m, p, max_len) : launch_tile<T, E, 128>(ctx, *m, p, max_len);
+    if (p.hd <= 64) return launch_tile<T, E, 64>(ctx, *m, p, max_len);
+    if constexpr (!std::is_same<T, float>::value)
+        if (p.hd > 128) return launch_tile<T, E, 256>(ctx, *m, p, max_len);
+    return launch_tile<T, E, 128>(ctx, *m, p, max_len);
 }
 
 int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &params, int q_type, const SeqKvDesc &kv, uint64_t max_len) {

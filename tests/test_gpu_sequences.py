@@ -452,3 +452,13 @@ def test_owned_pool_starts_zeroed_and_serves(env):
         ctx.sync()
         # both are the same sums in f32, in another order: 2^-20 of values below 4 (the split parts carry 2^-22)
         assert (out - want).abs().max().item() <= 4 * 2.0 ** -18
+
+
+@pytest.mark.parametrize("hd", [160, 256])
+@pytest.mark.parametrize("window", [0, 700])
+def test_wide_heads_in_chunks(env, hd, window):
+    """16-bit queries of head_dim above 128: one tile a CTA, keys split over a cluster or not."""
+    c = Case(*env, [(60, 3000)], 4, 1, hd, 64, "f16", seed=27)
+    c.check(c.run(window), window)
+    c = Case(*env, [(100, 300), (1, 50), (33, 33)], 6, 2, hd, 16, "f16", seed=28)
+    c.check(c.run(window, 20.0), window, 20.0)
