@@ -221,8 +221,8 @@ RCU_API int32_t rcu_paged_store(rcu_ctx *ctx, rcu_paged *pg, const rcu_seqs *seq
                                 const void *v_dev, uint32_t type, uint64_t ld);
 /* Causal grouped-query attention of the new tokens over their sequences' pages, the new tokens'
  * own keys and values (already stored) among them: any mix of single tokens and chunks in one
- * call. q_dev: n_tok rows of n_head * head_dim values (F32 or F16, already scaled by attn_scale),
- * ld_q apart; out_dev the same type, ld_out apart. window and softcap as in rcu_attention. Out rows
+ * call, at most 16384 sequences. q_dev: n_tok rows of n_head * head_dim values (F32 or F16, already scaled by attn_scale),
+ * ld_q apart; out_dev the same type, ld_out apart, and no part of q. window and softcap as in rcu_attention. Out rows
  * behind the last sequence stay as they were. Masked keys and values do not count, whatever they
  * hold. No workspace: calls may overlap on any streams. */
 RCU_API int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *seqs, const void *q_dev,
@@ -231,7 +231,7 @@ RCU_API int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu
 /* Causal grouped-query attention of whole prompts that lie one behind the other, without a cache:
  * rows cu[i] .. cu[i + 1] - 1 (device, n_seq + 1 offsets) attend among themselves. q (F32 or F16
  * over F16 keys and values, or BF16 over BF16; already scaled), k, v and out are rows ld_q / ld_kv /
- * ld_out values apart, so slices of a fused projection do. max_len: the longest prompt, 0 when
+ * ld_out values apart, so slices of a fused projection do; out must not overlap them. max_len: the longest prompt, 0 when
  * unknown (shapes the launch only). */
 RCU_API int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, uint64_t ld_q,
                                      const void *k_dev, const void *v_dev, uint32_t kv_elem, uint64_t ld_kv,

@@ -102,7 +102,8 @@ static int check_rows(rcu_ctx *ctx, const char *what, const void *p, uint64_t ld
 }
 static int check_batch(rcu_ctx *ctx, uint64_t n_tok, uint64_t n_seq) {
     if (n_tok == 0 || n_seq == 0) return set_err(ctx, RCU_ERR_RUNTIME, "empty batch");
-    if (n_tok > (1u << 30) || n_seq > (1u << 24)) return set_err(ctx, RCU_ERR_INVALID, "batch too large");
+    // every CTA looks for its sequence among all of them
+    if (n_tok > (1u << 30) || n_seq > (1u << 14)) return set_err(ctx, RCU_ERR_INVALID, "batch too large");
     return RCU_OK;
 }
 static int check_seqs(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s, SeqView *v) {
@@ -231,6 +232,7 @@ int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s
     if (int st = check_seqs(ctx, pg, seqs, &p.b)) return st;
     if (int st = check_heads(ctx, seqs->n_tok, n_head, pg->n_kv, pg->hd, window, softcap)) return st;
     if (type != T_F32 && type != T_F16) return set_err(ctx, RCU_ERR_UNSUPPORTED, "paged attention: queries are f32 or f16");
+    if (q_dev == out_dev) return set_err(ctx, RCU_ERR_INVALID, "paged attention: out must not be q");
     if (int st = check_rows(ctx, "paged attention: q", q_dev, ld_q, n_head * pg->hd, (int)type)) return st;
     if (int st = check_rows(ctx, "paged attention: out", out_dev, ld_out, n_head * pg->hd, (int)type)) return st;
     p.q = q_dev;
@@ -264,6 +266,8 @@ int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, u
     if (int st = check_heads(ctx, n_tok, n_head, n_head_kv, head_dim, window, softcap)) return st;
     if (!((q_type == T_F32 && kv_elem == T_F16) || (q_type == kv_elem && (q_type == T_F16 || q_type == T_BF16))))
         return set_err(ctx, RCU_ERR_UNSUPPORTED, "packed attention: queries are f32 or f16 over f16 keys and values, or bf16 over bf16");
+    if (q_dev == out_dev || k_dev == out_dev || v_dev == out_dev)
+        return set_err(ctx, RCU_ERR_INVALID, "packed attention: out must not be an input");
     if (int st = check_rows(ctx, "packed attention: q", q_dev, ld_q, n_head * head_dim, (int)q_type)) return st;
     if (int st = check_rows(ctx, "packed attention: k", k_dev, ld_kv, n_head_kv * head_dim, (int)kv_elem)) return st;
     if (int st = check_rows(ctx, "packed attention: v", v_dev, ld_kv, n_head_kv * head_dim, (int)kv_elem)) return st;

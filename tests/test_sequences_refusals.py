@@ -14,7 +14,7 @@ A = 0x10000  # an aligned address
 
 def packed(**kw):
     a = dict(q=A, q_type=F16, ld_q=256, k=A, v=A, kv=F16, ld_kv=128, cu=A, n_seq=2, n_tok=10, max_len=0, n_head=4, n_head_kv=2,
-             hd=64, window=0, softcap=0.0, out=A, ld_out=256)
+             hd=64, window=0, softcap=0.0, out=2 * A, ld_out=256)
     assert set(kw) <= set(a)
     a.update(kw)
     return _lib.load().rcu_packed_attention(None, a["q"], a["q_type"], a["ld_q"], a["k"], a["v"], a["kv"], a["ld_kv"], a["cu"],
@@ -31,6 +31,7 @@ def packed(**kw):
     (dict(q_type=BF16), UNSUPPORTED), (dict(kv=F32, q_type=F32), UNSUPPORTED), (dict(kv=BF16), UNSUPPORTED), (dict(q_type=2), UNSUPPORTED),
     (dict(q=A + 2), INVALID), (dict(k=A + 8), INVALID), (dict(v=A + 8), INVALID), (dict(out=A + 8), INVALID),
     (dict(ld_q=255), INVALID), (dict(ld_q=260), INVALID), (dict(ld_kv=120), INVALID), (dict(ld_kv=132), INVALID), (dict(ld_out=248), INVALID),
+    (dict(out=A), INVALID), (dict(n_seq=16385, n_tok=20000), INVALID),
     (dict(n_tok=1 << 30, n_head=4096, n_head_kv=1, ld_q=1 << 19, ld_out=1 << 19), INVALID),
     (dict(), INVALID),  # nothing but the context is missing
 ])
