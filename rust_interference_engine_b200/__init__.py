@@ -403,24 +403,31 @@ def _elem(x) -> int:
     return ty
 
 
+def _elsewhere(ctx: Context, x, what: str):
+    return ValueError(f"{what}: expected a CUDA tensor" if x.get_device() < 0 else
+                      f"{what}: on device {x.get_device()}, the context is on {ctx.device}")
+
+
 def _on(ctx: Context, x, what: str) -> int:
     """Device address of a tensor that must live on the context's device."""
-    if not x.is_cuda:
-        raise ValueError(f"{what}: expected a CUDA tensor")
-    if x.get_device() != ctx.device:
-        raise ValueError(f"{what}: on device {x.get_device()}, the context is on {ctx.device}")
+    if x.get_device() != ctx.device:  # -1: not a CUDA tensor
+        raise _elsewhere(ctx, x, what)
     return x.data_ptr()
 
 
 def _rows(ctx: Context, x, n: int, width: int, what: str):
     """(address, type, row stride) of n rows of `width` values; the rows may be slices of wider
-    ones, their values must be contiguous."""
+    ones, their values must be contiguous. (One call for each tensor of a small launch: nothing in
+    here is done twice.)"""
     if x.shape != (n, width):
         raise ValueError(f"{what}: expected {n} x {width} values, not {tuple(x.shape)}")
     ld, step = x.stride()
     if step != 1 and width > 1:
         raise ValueError(f"{what}: the values of a row must be contiguous")
-    return _on(ctx, x, what), _elem(x), ld if n > 1 else max(ld, width)
+    if x.get_device() != ctx.device:
+        raise _elsewhere(ctx, x, what)
+    ty = _ELEM.get(x.dtype)
+    return x.data_ptr(), _elem(x) if ty is None else ty, ld if n > 1 else max(ld, width)
 
 
 def _vector(ctx: Context, x, dtype: str, shape, what: str) -> int:
@@ -428,7 +435,9 @@ def _vector(ctx: Context, x, dtype: str, shape, what: str) -> int:
         _torch_types()
     if x.dtype is not _DTYPE[dtype] or x.shape != shape or not x.is_contiguous():
         raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, not {x.dtype} {tuple(x.shape)}")
-    return _on(ctx, x, what)
+    if x.get_device() != ctx.device:
+        raise _elsewhere(ctx, x, what)
+    return x.data_ptr()
 
 
 class SeqBatch:
