@@ -139,12 +139,13 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
     constexpr int kChunks = HDP / 64, kTiles = C::kTiles, kTlRows = C::kRows, kTlSoftWarps = C::kSoftWarps;
     extern __shared__ __align__(1024) uint8_t tl_raw[];  // swizzled tiles start on 1024-byte boundaries
     S &sm = *reinterpret_cast<S *>(tl_raw);
-    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    constexpr uint32_t kMmaWarp = 0, kLoadWarp = 1, kSoft0 = 4;  // warps by role
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), sw = warp - kSoft0, lane = threadIdx.x & 31;
     const uint32_t rank = p.splits > 1 ? cluster_ctarank() : 0;
     const uint32_t item = blockIdx.x / p.splits, kvh = item % p.n_kv, ti = p.n_tiles - 1 - item / p.n_kv;
     // what needs no input first: tensor memory, and the barriers by the warp that uses them at once
-    if (warp == kTlSoftWarps + 1) tmem_alloc<512>(&sm.tmem);
-    if (warp == kTlSoftWarps) {
+    if (warp == kMmaWarp) tmem_alloc<512>(&sm.tmem);
+    if (warp == kLoadWarp) {
         if (lane == 0) {
             for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
             for (int t = 0; t < kTiles; t++)
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
     SeqSpan sp;
     uint32_t tile;
     if (!seq_find_tile(p.b, p.group, kTlRows, ti, &sp, &tile)) {  // the same for the whole cluster
-        if (warp == kTlSoftWarps + 1) tmem_free<512>(sm.tmem);
+        if (warp == kMmaWarp) tmem_free<512>(sm.tmem);
         return;
     }
     const uint32_t row0 = tile * kTlRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kTlRows);
@@ -178,11 +179,11 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
         }
     }
     uint8_t *ring = sm.data + C::kQ;
-    if (warp < kTlSoftWarps) {
-        const uint32_t t = warp >> 3;
+    if (warp >= kSoft0) {
+        const uint32_t t = sw >> 3;
         if (t < n_tiles) {  // Q into shared memory (K-major, 128-byte swizzle), whole rows by neighbouring lanes
             uint8_t *q = sm.data + t * C::kParts * C::kPart;
-            const uint32_t w8 = warp & 7;
+            const uint32_t w8 = sw & 7;
             auto source = [&](uint32_t i) {  // row i of the tile
                 const uint32_t rr = row0 + min(128 * t + i, n_rows - 1);
                 const uint32_t tk = div_group(p, rr);
@@ -250,11 +251,11 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
         tc_fence_after();
         tmem = sm.tmem;
     };
-    if (warp != kTlSoftWarps) meet();  // the producer has its copies on their way first
-    if (warp >= kTlSoftWarps) {
+    if (warp != kLoadWarp) meet();  // the producer has its copies on their way first
+    if (warp < kSoft0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
     }
-    if (warp == kTlSoftWarps) {  // ---- producer ----
+    if (warp == kLoadWarp) {  // ---- producer ----
         bool met = false;
         const uint32_t box = p.b.pages ? min(1u << p.b.page_shift, (uint32_t)kTlBlk) : (uint32_t)kTlBlk;
         const uint32_t n_box = kTlBlk / box;  // boxes of rows per block (8 at most, pages of 16)
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
         // every copy has landed before this CTA goes on to its end
         for (uint32_t i = it > C::kStages ? it - C::kStages : 0; i < it; i++)
             mbar_wait_sleep(&sm.full[i % C::kStages], (i / C::kStages) & 1, p.b.err, ERR_TIMEOUT_FULL);
-    } else if (warp == kTlSoftWarps + 1) {  // ---- MMA ----
+    } else if (warp == kMmaWarp) {  // ---- MMA ----
         // The whole warp walks the blocks and one elected lane issues: the loop's state is the same in
         // every lane (taken from lane 0), so the descriptors stay in uniform registers. Issued from a
         // branch of lane 0 alone, an MMA cost 107 cycles of moves into them, against 64 of work.
@@ -299,51 +300,66 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
         const uint32_t tm = uni((int32_t)tmem);
         const uint64_t dq = sw128_desc(sm.data), dk = sw128_desc(ring), dv = sw128_desc_mn(ring, kTlBlk * 128);
         const bool elected = elect_one();
+        // After a wait that ran out (the result is void) the walk goes on without waiting.
         bool ok = true;
         auto wait = [&](uint64_t *bar, uint32_t parity) {
-            ok = __all_sync(0xffffffffu, ok && mbar_wait_spin(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
+            bool there = false;
+#pragma unroll 1
+            for (int i = 0; i < 64 && !there; i++) there = __all_sync(0xffffffffu, mbar_test(bar, parity));
+            if (!there && ok) ok = __all_sync(0xffffffffu, mbar_wait_spin(bar, parity, p.b.err, ERR_TIMEOUT_FULL));
             tc_fence_after();
-            return ok;
         };
-        uint32_t np[2] = {0, 0};
+        uint32_t np = 0;                          // bit t: parity of tile t's P
         uint32_t sk = 0, pk = 0, sv = 1, pv = 0;  // ring stage and parity of K(j), V(j - 1)
-        for (int32_t j = 0; j <= n_blk && ok; j++) {
-            const bool last = j == n_blk;
-            if (j > 0) {
-                wait(&sm.full[sv], pv);
-                if (j * kTlBlk > n_keys) {  // rows behind the last key hold anything: 0 * v must stay 0
-                    uint8_t *v = ring + sv * C::kStage;
-                    for (uint32_t i = (uint32_t)(n_keys - (j - 1) * kTlBlk) * 8 + lane; i < kTlBlk * 8; i += 32)
+        // K and V blocks take turns in the ring
+        auto next = [](uint32_t &s, uint32_t &par) {
+            s += 2;
+            if (s >= (uint32_t)C::kStages) s -= C::kStages, par ^= 1;
+        };
+        auto wait_v = [&](int32_t j, uint32_t s, uint32_t par) {  // V(j)
+            wait(&sm.full[s], par);
+            if ((j + 1) * kTlBlk > n_keys) {  // rows behind the last key hold anything: 0 * v must stay 0
+                uint8_t *v = ring + s * C::kStage;
+#pragma unroll 1
+                for (uint32_t i = (uint32_t)(n_keys - j * kTlBlk) * 8 + lane; i < kTlBlk * 8; i += 32)
 #pragma unroll
-                        for (int c = 0; c < kChunks; c++) *reinterpret_cast<uint4 *>(v + c * (kTlBlk * 128) + i * 16) = make_uint4(0, 0, 0, 0);
-                    fence_async_smem();
-                    __syncwarp();
-                }
+                    for (int c = 0; c < kChunks; c++) *reinterpret_cast<uint4 *>(v + c * (kTlBlk * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_async_smem();
+                __syncwarp();
             }
-            if (!last) wait(&sm.full[sk], pk);
-#pragma unroll
+        };
+        // Where the ring has room for them, the next blocks are waited for while the tensor core is at
+        // work, not between a tile's P and its products: every step of this warp there is lost time.
+        constexpr bool kEarlyV = C::kStages >= 3, kEarlyK = C::kStages >= 4;
+        if (n_blk > 0) wait(&sm.full[sk], pk);
+        for (int32_t j = 0; j <= n_blk; j++) {
+            const bool last = j == n_blk;
+            if (!kEarlyV && j > 0) wait_v(j - 1, sv, pv);
+            if (!kEarlyK && j > 0 && !last) wait(&sm.full[sk], pk);
+#pragma unroll 1
             for (int t = 0; t < kTiles; t++) {
                 const uint32_t ts = tm + 128 * t, to = tm + 128 * kTiles + HDP * t;
                 const int32_t b = t ? b1 : b0, e = t ? e1 : e0;
-                if (j - 1 >= b && j - 1 < e && ok) {  // O_t += P_t V(j - 1)
+                if (j > b && j <= e) {  // O_t += P_t V(j - 1)
                     const uint64_t v = dv + sv * (C::kStage >> 4);
-#pragma unroll
+#pragma unroll 1
                     for (int half = 0; half < 2; half++) {  // keys 64 half .. 64 half + 63
-                        if (!wait(half ? &sm.p_full[t] : &sm.p_half[t], np[t] & 1)) break;
+                        wait(half ? &sm.p_full[t] : &sm.p_half[t], np >> t & 1);
                         if (elected) {
 #pragma unroll
-                            for (int kk = 4 * half; kk < 4 * half + 4; kk++) {
-                                const uint32_t a = ts + 16 * kk;
-                                tl_mma_ts(to, a, v + (2048 >> 4) * kk, kIdO, kk > 0 || (!kSplit && j - 1 > b));
-                                if constexpr (kSplit) tl_mma_ts(to, a + 8, v + (2048 >> 4) * kk, kIdO, true);
+                            for (int kk = 0; kk < 4; kk++) {
+                                const uint32_t a = ts + 64 * half + 16 * kk;
+                                const uint64_t vk = v + (2048 >> 4) * (4 * half + kk);
+                                tl_mma_ts(to, a, vk, kIdO, kk > 0 || half > 0 || (!kSplit && j - 1 > b));
+                                if constexpr (kSplit) tl_mma_ts(to, a + 8, vk, kIdO, true);
                             }
                         }
                     }
-                    np[t]++;
+                    np ^= 1u << t;
                     if (j == e && elected) mma_commit(&sm.o_done[t]);
                 }
                 if (t == kTiles - 1 && j > 0 && elected) mma_commit(&sm.empty[sv]);
-                if (j >= b && j < e && ok) {  // S_t = Q_t K(j)^T
+                if (j >= b && j < e) {  // S_t = Q_t K(j)^T
                     if (elected) {
                         const uint64_t k = dk + sk * (C::kStage >> 4), q = dq + t * ((C::kParts * C::kPart) >> 4);
                         if constexpr (kSplit) {
@@ -362,26 +378,27 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
                     }
                     __syncwarp();
                 }
+                if (t == 0 && !last) {
+                    uint32_t s = sv, par = pv;
+                    if (j > 0) next(s, par);
+                    if (kEarlyV) wait_v(j, s, par);
+                    s = sk, par = pk;
+                    next(s, par);
+                    if (kEarlyK && j + 1 < n_blk) wait(&sm.full[s], par);
+                }
             }
             if (!last && elected) mma_commit(&sm.empty[sk]);
-            // K and V blocks take turns in the ring
-            auto next = [](uint32_t &s, uint32_t &par) {
-                s += 2;
-                if (s >= (uint32_t)C::kStages) s -= C::kStages, par ^= 1;
-            };
             if (j > 0) next(sv, pv);
             next(sk, pk);
         }
         if (elected) {
-            if (!ok)
-                for (int t = 0; t < kTiles; t++) mma_commit(&sm.o_done[t]);
-            mma_commit(&sm.done);  // every MMA issued, on an early end too
+            mma_commit(&sm.done);  // every MMA issued
         }
         __syncwarp();
         mbar_wait_sleep(&sm.done, 0, p.b.err, ERR_TIMEOUT_DRAIN);
-    } else if (warp < kTlSoftWarps) {  // ---- softmax: row r of tile t, keys 64 h .. 64 h + 63 of each block ----
+    } else if (warp >= kSoft0) {  // ---- softmax: row r of tile t, keys 64 h .. 64 h + 63 of each block ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
-        const uint32_t t = warp >> 3, h = (warp >> 2) & 1, r = threadIdx.x & 127, tr = 128 * t + r;
+        const uint32_t t = sw >> 3, h = (sw >> 2) & 1, r = threadIdx.x & 127, tr = 128 * t + r;
         const uint32_t pair = 1 + 4 * t + (warp & 3);    // barrier of the two warps that share these rows
         const uint32_t lanes = (32 * (warp & 3)) << 16;  // their TMEM lanes
         const uint32_t ts = tmem + 128 * t + 64 * h + lanes, to = tmem + 128 * kTiles + HDP * t + HDP / 2 * h + lanes;
@@ -584,7 +601,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
                 const uint32_t ch = lane % kLanes;
 #pragma unroll 4
                 for (uint32_t k = 0; k < 16 / kRows; k++) {
-                    const uint32_t i = ((warp & 7) * (16 / kRows) + k) * kRows + lane / kLanes;
+                    const uint32_t i = ((sw & 7) * (16 / kRows) + k) * kRows + lane / kLanes;
                     if (128 * t + i >= n_rows || ch * kPer >= p.hd) continue;
                     const uint32_t rr = row0 + 128 * t + i;
                     const uint32_t tk = div_group(p, rr);
@@ -623,8 +640,8 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
         cluster_sync_all();
         // weight of each CTA's part of row i: 2^(m_c - max m) / sum_c l_c 2^(m_c - max m)
         float *wt = reinterpret_cast<float *>(sm.data + kTlRows * HDP * 4);
-        if (threadIdx.x < n_rows) {
-            const uint32_t i = threadIdx.x, am = smem_u32(&sm.mx[0][i]), al = smem_u32(&sm.mx[1][i]);
+        if (threadIdx.x - 32 * kSoft0 < n_rows) {
+            const uint32_t i = threadIdx.x - 32 * kSoft0, am = smem_u32(&sm.mx[0][i]), al = smem_u32(&sm.mx[1][i]);
             float mc[kTlMaxCluster], lc[kTlMaxCluster], M = -INFINITY, L = 0.0f;
 #pragma unroll
             for (int c = 0; c < kTlMaxCluster; c++) {
@@ -647,7 +664,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
         constexpr int kVec = HDP / 4, kLn = kVec < 32 ? kVec : 32, kPerRow = kVec / kLn;  // 16-byte chunks of a row, lanes, chunks a lane
         const uint32_t step = p.splits * kTlSoftWarps * 32 / kLn;
 #pragma unroll 2
-        for (uint32_t i = (rank * kTlSoftWarps + warp) * (32 / kLn) + lane / kLn; i - lane / kLn < n_rows; i += step) {
+        for (uint32_t i = (rank * kTlSoftWarps + sw) * (32 / kLn) + lane / kLn; i - lane / kLn < n_rows; i += step) {
             const bool in = i < n_rows;
             const uint32_t rr = row0 + (in ? i : 0), tk = div_group(p, rr), gq = rr - tk * p.group;
             T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + tk) * p.ld_out + (uint64_t)(kvh * p.group + gq) * p.hd;
@@ -685,7 +702,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
     }
     if (p.splits > 1) cluster_sync_all();
     else __syncthreads();
-    if (warp == kTlSoftWarps + 1) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_free<512>(tmem);
     }
