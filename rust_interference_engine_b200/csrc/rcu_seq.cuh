@@ -111,12 +111,6 @@ __device__ __forceinline__ uint32_t seq_kv_row(const SeqView &b, const SeqSpan &
     return ((pg * n_kv + kvh) << b.page_shift) + (pos & ((1u << b.page_shift) - 1));
 }
 
-// x, of which the compiler knows nothing: what is computed from it is not kept from before.
-__device__ __forceinline__ uint32_t fresh(uint32_t x) {
-    asm volatile("" : "+r"(x));
-    return x;
-}
-
 // ---- elements ---------------------------------------------------------------------------------
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
@@ -211,7 +205,7 @@ __device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity, u
     }
 }
 
-// Whether the phase is complete, without suspending: what a try_wait answers in 200 cycles.
+// Whether the phase is complete, without suspending the thread.
 __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
