@@ -2,8 +2,9 @@
 // whole prompts) on the 5th-generation tensor cores. Formula and batch as in rcu_attn_seq.cu.
 //
 // A CTA takes 256 query rows (token, head of the group) of one sequence and KV head as two tiles of
-// 128 rows (head_dim above 128: one tile, since O fills tensor memory), and walks the attended keys in
-// blocks of 128:
+// 128 rows, or 128 as one, and walks the attended keys in blocks of 128 (one tile: 16-bit queries
+// whose CTAs are short, two CTAs to an SM, so that one's start and end run beside the other's blocks;
+// head_dim above 128, since O fills tensor memory):
 //   * warp 0     owns tensor memory; one lane issues S_t = Q_t K^T (M 128, N 128) and O_t += P_t V
 //                (P read from tensor memory, V in its own layout as an MN-major operand);
 //   * warp 1     producer: K and V blocks by tiled TMA (128-byte swizzle) into a ring of stages; a
@@ -13,7 +14,7 @@
 //                keys of the block and one for the others: S out of tensor memory, mask, running
 //                maximum (the two exchange theirs) and sum in f32, P = 2^(s - m) back as packed
 //                16-bit values over S, each half handed on by itself.
-// While one tile's warps are at their softmax, the tensor core works on the other tile.
+// While one tile's warps are at their softmax, the tensor core works on the other tile (CTA).
 // 16-bit queries: O stays in tensor memory; it is rescaled only when a row's maximum has grown by
 // more than 2^kTlLazy since its last rescale (p then is at most 2^(kTlLazy + kTlShift)).
 // f32 queries: q (scaled by a power of two per row) and p are each split into two f16 parts, so each
@@ -42,27 +43,30 @@ constexpr int kTlBlk = kSeqTileBox;  // keys per block
 constexpr int kTlMaxCluster = 8;
 constexpr float kTlLazy = 8.0f, kTlShift = 7.0f;
 
-template <int HDP, bool SPLIT>
+template <int HDP, bool SPLIT, int TILES>
 struct TlCfg {
-    static constexpr int kTiles = HDP == 256 ? 1 : 2;
+    static_assert(TILES == 1 || HDP < 256, "O of two tiles does not fit tensor memory");
+    static constexpr int kTiles = TILES;
+    static constexpr int kPerSm = TILES == 1 && HDP < 256 ? 2 : 1;  // CTAs on an SM
+    static constexpr int kTmem = 512 / kPerSm;               // tensor memory columns: 128 for S and HDP for O, each tile
     static constexpr int kRows = 128 * kTiles;               // query rows per CTA
     static constexpr int kSoftWarps = 8 * kTiles;
     static constexpr int kThreads = 32 * (kSoftWarps + 4);   // a warpgroup for the MMA issuer and the producer
-    // registers a thread: the first warpgroup gives its own up (4 x 112 + 32 = 5 x 96, or 2 x 224 + 56 =
-    // 3 x 168, the launch's)
-    static constexpr int kRegsSoftmax = kTiles == 2 ? 112 : 224, kRegsOther = kTiles == 2 ? 32 : 56;
+    // registers a thread: the first warpgroup gives its own up (4 x 112 + 32 = 5 x 96, 2 x 104 + 32 = 3 x 80
+    // or 2 x 224 + 56 = 3 x 168, the launch's)
+    static constexpr int kRegsSoftmax = kTiles == 2 ? 112 : kPerSm == 2 ? 104 : 224, kRegsOther = kTiles == 2 || kPerSm == 2 ? 32 : 56;
     static constexpr int kPart = 128 * HDP * 2;              // one tile's Q (one part of it)
     static constexpr int kParts = SPLIT ? 2 : 1;
     static constexpr int kQ = kTiles * kParts * kPart;
     static constexpr int kStage = kTlBlk * HDP * 2;          // one K or V block
-    static constexpr int kStages = HDP == 64 ? 8 : HDP == 256 ? 2 : SPLIT ? 3 : 5;
+    static constexpr int kStages = kPerSm == 2 ? (HDP == 64 ? 5 : 2) : HDP == 64 ? 8 : HDP == 256 ? 2 : SPLIT ? 3 : 5;
     static constexpr int kData = kQ + kStages * kStage;
     static_assert(kData >= kRows * HDP * 4 + kTlMaxCluster * kRows * 4, "the joined O and its weights overlay Q and the ring");
-    static_assert(!(SPLIT && HDP == 256), "Q's two parts leave no room for a ring");
+    static_assert(!SPLIT || TILES == 2, "Q's two parts leave too little room for a ring");
 };
-template <int HDP, bool SPLIT>
+template <int HDP, bool SPLIT, int TILES>
 struct TlSmem {
-    using C = TlCfg<HDP, SPLIT>;
+    using C = TlCfg<HDP, SPLIT, TILES>;
     uint8_t data[C::kData];  // Q, then the ring; at the end O and its weights when a cluster joins
     float mx[2][C::kRows];   // [half of the block's keys]: row maxima; at the end the row's m and l
     uint64_t full[C::kStages], empty[C::kStages], s_full[2], p_half[2], p_full[2], o_done[2], done;
@@ -128,13 +132,13 @@ __device__ __forceinline__ TlSpan tl_span(const SeqAttnParams &p, const SeqSpan 
     return {p.window > 0 ? max(a - (int32_t)p.window + 1, 0) / kTlBlk : 0, b / kTlBlk + 1};
 }
 
-template <typename T, typename E, int HDP>
-__global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kThreads, 1) k_attn_tile(const __grid_constant__ CUtensorMap mk,
+template <typename T, typename E, int HDP, int TILES>
+__global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILES>::kThreads, TlCfg<HDP, std::is_same<T, float>::value, TILES>::kPerSm) k_attn_tile(const __grid_constant__ CUtensorMap mk,
                                                              const __grid_constant__ CUtensorMap mv,
                                                              const __grid_constant__ SeqAttnParams p) {
     constexpr bool kSplit = std::is_same<T, float>::value;
-    using C = TlCfg<HDP, kSplit>;
-    using S = TlSmem<HDP, kSplit>;
+    using C = TlCfg<HDP, kSplit, TILES>;
+    using S = TlSmem<HDP, kSplit, TILES>;
     constexpr int kChunks = HDP / 64, kTiles = C::kTiles, kTlRows = C::kRows, kTlSoftWarps = C::kSoftWarps;
     extern __shared__ __align__(1024) uint8_t tl_raw[];  // swizzled tiles start on 1024-byte boundaries
     S &sm = *reinterpret_cast<S *>(tl_raw);
@@ -143,7 +147,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
     const uint32_t rank = p.splits > 1 ? cluster_ctarank() : 0;
     const uint32_t item = blockIdx.x / p.splits, kvh = item % p.n_kv, ti = p.n_tiles - 1 - item / p.n_kv;
     // what needs no input first: tensor memory, and the barriers by the warp that uses them at once
-    if (warp == kMmaWarp) tmem_alloc<512>(&sm.tmem);
+    if (warp == kMmaWarp) tmem_alloc<C::kTmem>(&sm.tmem);
     if (warp == kLoadWarp) {
         if (lane == 0) {
             for (int s = 0; s < C::kStages; s++) mbar_init(&sm.full[s], 1), mbar_init(&sm.empty[s], 1);
@@ -159,7 +163,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
     SeqSpan sp;
     uint32_t tile;
     if (!seq_find_tile(p.b, p.group, kTlRows, ti, &sp, &tile)) {  // the same for the whole cluster
-        if (warp == kMmaWarp) tmem_free<512>(sm.tmem);
+        if (warp == kMmaWarp) tmem_free<C::kTmem>(sm.tmem);
         return;
     }
     const uint32_t row0 = tile * kTlRows, n_rows = min(sp.n_new * p.group - row0, (uint32_t)kTlRows);
@@ -704,7 +708,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
     else __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        tmem_free<512>(tmem);
+        tmem_free<C::kTmem>(tmem);
     }
     if (p.splits > 1) cluster_sync_all();
 }
@@ -712,28 +716,74 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value>::kTh
 // ---- host ---------------------------------------------------------------------------------------
 bool attention_tile_ok(uint64_t hd, int q_type) { return hd <= 128 || q_type != T_F32; }
 
-template <typename T, typename E, int HDP>
-static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint64_t max_len) {
-    using C = TlCfg<HDP, std::is_same<T, float>::value>;
-    constexpr size_t smem = sizeof(TlSmem<HDP, std::is_same<T, float>::value>);
-    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, C::kRows);
-    static_assert(smem <= 232448, "shared memory of one CTA");
-    const uint64_t items = (uint64_t)p.n_tiles * p.n_kv, span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + C::kRows) : max_len;
-    // CTAs per tile by the time they take, in blocks of keys: each its share and, for its start, its end
-    // and the join, about 5 (alone) or 7 more; the last wave is half full on average. Sequences of
-    // different lengths count as 0.6 of the longest. (16 sequences of 250 .. 5000 keys, two chunks among
-    // them: 79 us alone, 64 us by two, 88 us by four; one chunk over 12,800 keys: 177 us by two, 186 by four.)
+// How many CTAs share a tile's keys, by the time that the launch takes in blocks of keys (about 1.8 us
+// each): a CTA's share of the blocks and, for its start and end, 5 more (7 with the join). Two CTAs on
+// an SM hide a part of those (3.5 and 6), but bring each block in twice and take 9 % longer. A launch
+// that does not fill the device takes as long as its longest tile. Beyond that tiles of unequal
+// lengths share the SMs evenly and end a fifth of a tile late, equal ones run in whole waves. The
+// average tile of a prompt over itself has half the keys, one of several sequences 0.6 of the longest.
+// (128 rows over 8128 keys, 8 KV heads, f16: two tiles a CTA 123, 71, 43, 57 us by 1, 2, 4, 8 CTAs,
+// where the device does not hold all clusters of 8; one tile 116, 65, 39, 30. 16 sequences of 250 ..
+// 5333 keys, two chunks of 333 rows among them: 75, 64, 87, 156 and 107, 59, 67, 109. 16 prompts of 65
+// .. 2047 tokens: 295 and 278 by one CTA. One prompt of 8192: 480 and 510. 512 rows over 12,800 keys:
+// 190, 106, 118, 187 and 181, 111, 120, 151.)
+struct TlPlan {
+    uint32_t splits;
+    double cost;
+};
+template <typename T, typename E, int HDP, int TILES>
+static int plan_tile(rcu_ctx *ctx, const SeqAttnParams &p, uint64_t max_len, TlPlan *plan) {
+    using C = TlCfg<HDP, std::is_same<T, float>::value, TILES>;
+    constexpr size_t smem = sizeof(TlSmem<HDP, std::is_same<T, float>::value, TILES>);
+    const double items = (double)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, C::kRows) * p.n_kv;
+    const uint64_t span = p.window > 0 ? std::min<uint64_t>(max_len, p.window + C::kRows) : max_len;
     const double blocks = (double)((span + kTlBlk - 1) / kTlBlk);
-    uint32_t cs = 1;
-    double best = 0.0;
-    for (uint32_t c = 1; c <= kTlMaxCluster && (c == 1 || blocks >= 2.0 * c); c *= 2) {
-        const double f = (double)items * c / ctx->num_sms, waves = f <= 1.0 ? 1.0 : p.b.n_seq > 1 ? 0.6 * f + 0.5 : std::ceil(f);
-        const double cost = waves * (blocks / c + (c == 1 ? 5.0 : 7.0));
-        if (c == 1 || cost < best) best = cost, cs = c;
+    const double part = p.window > 0 ? 0.0 : std::min(1.0, (double)p.b.n_tok / ((double)p.b.n_seq * max_len));
+    const double mean = (p.b.n_seq > 1 ? 0.6 : 1.0) * (1.0 - 0.5 * part);  // of `blocks`
+    *plan = {1, 0.0};
+    for (int e = 0; 1 << e <= kTlMaxCluster && (e == 0 || blocks >= 2.0 * (1 << e)); e++) {
+        int slots = ctx->num_sms * C::kPerSm;
+        if (e > 0 && C::kPerSm == 1) {
+            if (int st = cluster_slots<k_attn_tile<T, E, HDP, TILES>>(ctx, C::kThreads, smem, e, &slots)) return st;
+        } else if (e > 0) {  // n SMs hold as many clusters of 2^e with two CTAs each as of half the size with one
+            using W = TlCfg<HDP, false, HDP == 256 ? 1 : 2>;
+            constexpr size_t wide = sizeof(TlSmem<HDP, false, W::kTiles>);
+            if (e == 1) slots = ctx->num_sms;
+            else if (int st = cluster_slots<k_attn_tile<T, E, HDP, W::kTiles>>(ctx, W::kThreads, wide, e - 1, &slots)) return st;
+        }
+        const double f = items / slots, ends = C::kPerSm == 2 ? (e ? 6.0 : 3.5) : (e ? 7.0 : 5.0);
+        const double longest = blocks / (1 << e) + ends, usual = blocks * mean / (1 << e) + ends;
+        double cost = f <= 1.0 ? longest : std::max(longest, (mean < 0.8 ? f + 0.2 : std::ceil(f)) * usual);
+        if (C::kPerSm == 2) cost *= 1.09;
+        if (e == 0 || cost < plan->cost) *plan = {1u << e, cost};
     }
-    p.splits = cs;
-    if (items * cs > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
-    return launch_cluster_k<k_attn_tile<T, E, HDP>>(ctx, (uint32_t)(items * cs), C::kThreads, smem, cs, m.k, m.v, p);
+    return RCU_OK;
+}
+
+template <typename T, typename E, int HDP, int TILES>
+static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint32_t splits) {
+    using C = TlCfg<HDP, std::is_same<T, float>::value, TILES>;
+    constexpr size_t smem = sizeof(TlSmem<HDP, std::is_same<T, float>::value, TILES>);
+    static_assert(smem <= 232448 && (smem + 1024) * C::kPerSm <= 233472, "shared memory of one CTA, of an SM");
+    p.n_tiles = (uint32_t)seq_tiles_bound(p.b.n_tok, p.b.n_seq, p.group, C::kRows);
+    p.splits = splits;
+    const uint64_t grid = (uint64_t)p.n_tiles * p.n_kv * splits;
+    if (grid > 0x7fffffffull) return set_err(ctx, RCU_ERR_INVALID, "attention: too many work tiles");
+    return launch_cluster_k<k_attn_tile<T, E, HDP, TILES>>(ctx, (uint32_t)grid, C::kThreads, smem, splits, m.k, m.v, p);
+}
+
+// The form with the smaller cost. f32 queries and head_dim above 128 have one form each: their Q or O
+// leaves no room for the other.
+template <typename T, typename E, int HDP>
+static int launch_tile_form(rcu_ctx *ctx, const SeqKvMaps &m, const SeqAttnParams &p, uint64_t max_len) {
+    TlPlan one{1, 1.0}, two{1, 0.0};
+    if constexpr (HDP < 256)
+        if (int st = plan_tile<T, E, HDP, 2>(ctx, p, max_len, &two)) return st;
+    if constexpr (!std::is_same<T, float>::value) {
+        if (int st = plan_tile<T, E, HDP, 1>(ctx, p, max_len, &one)) return st;
+        if (HDP == 256 || one.cost < two.cost) return launch_tile<T, E, HDP, 1>(ctx, m, p, one.splits);
+    }
+    if constexpr (HDP < 256) return launch_tile<T, E, HDP, 2>(ctx, m, p, two.splits);
 }
 
 template <typename T, typename E>
@@ -741,10 +791,10 @@ static int launch_tile_hd(rcu_ctx *ctx, SeqAttnParams &p, const SeqKvDesc &kv, u
     SeqKvMaps room;
     const SeqKvMaps *m;
     if (int st = seq_pick_maps(ctx, p, kv, kSeqTileBox, kv.tile, &room, &m)) return st;
-    if (p.hd <= 64) return launch_tile<T, E, 64>(ctx, *m, p, max_len);
+    if (p.hd <= 64) return launch_tile_form<T, E, 64>(ctx, *m, p, max_len);
     if constexpr (!std::is_same<T, float>::value)
-        if (p.hd > 128) return launch_tile<T, E, 256>(ctx, *m, p, max_len);
-    return launch_tile<T, E, 128>(ctx, *m, p, max_len);
+        if (p.hd > 128) return launch_tile_form<T, E, 256>(ctx, *m, p, max_len);
+    return launch_tile_form<T, E, 128>(ctx, *m, p, max_len);
 }
 
 int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &params, int q_type, const SeqKvDesc &kv, uint64_t max_len) {

@@ -338,10 +338,9 @@ inline int seq_pick_maps(rcu_ctx *ctx, const SeqAttnParams &p, const SeqKvDesc &
     *use = room;
     return seq_kv_maps(ctx, kv, p.hd, p.n_kv, box, room);
 }
-// Clusters of cs CTAs, programmatic dependent launch as launch_k. The kernel's attributes are set by
-// its first launch on a device.
-template <auto Kern, typename... Args>
-inline int launch_cluster_k(rcu_ctx *ctx, uint32_t grid, uint32_t threads, size_t smem, uint32_t cs, const Args &...args) {
+// Shared memory and cluster attributes of a kernel, set by its first use on a device.
+template <auto Kern>
+inline int prepare_cluster_k(rcu_ctx *ctx, size_t smem) {
     static std::atomic<uint64_t> ready{0};  // devices, of the first 64
     const uint64_t bit = 1ull << (ctx->device & 63);
     if (ctx->device >= 64 || !(ready.load(std::memory_order_acquire) & bit)) {
@@ -351,6 +350,34 @@ inline int launch_cluster_k(rcu_ctx *ctx, uint32_t grid, uint32_t threads, size_
         RCU_CUDA_TRY(ctx, cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         ready.fetch_or(bit, std::memory_order_release);
     }
+    return RCU_OK;
+}
+// Clusters of 2^e CTAs (e below 4) of a kernel that the device runs at the same time.
+template <auto Kern>
+inline int cluster_slots(rcu_ctx *ctx, uint32_t threads, size_t smem, int e, int *slots) {
+    static std::atomic<int> known[64][4];
+    const bool keep = ctx->device < 64;
+    if (keep && (*slots = known[ctx->device][e].load(std::memory_order_relaxed)) > 0) return RCU_OK;
+    if (int st = prepare_cluster_k<Kern>(ctx, smem)) return st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1u << e;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << e);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    RCU_CUDA_TRY(ctx, cudaOccupancyMaxActiveClusters(slots, Kern, &cfg));
+    *slots = std::max(*slots, 1);
+    if (keep) known[ctx->device][e].store(*slots, std::memory_order_relaxed);
+    return RCU_OK;
+}
+// Clusters of cs CTAs, programmatic dependent launch as launch_k.
+template <auto Kern, typename... Args>
+inline int launch_cluster_k(rcu_ctx *ctx, uint32_t grid, uint32_t threads, size_t smem, uint32_t cs, const Args &...args) {
+    if (int st = prepare_cluster_k<Kern>(ctx, smem)) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
