@@ -18,7 +18,7 @@
 // 16-bit queries: O stays in tensor memory; it is rescaled only when a row's maximum has grown by
 // more than 2^kTlLazy since its last rescale (p then is at most 2^(kTlLazy + kTlShift)).
 // f32 queries: q (scaled by a power of two per row) and p are each split into two f16 parts, so each
-// product is two MMAs; O is added up in registers block by block, because a long chain of additions
+// product is two MMAs (head_dim above 128: Q's low part in the tensor memory that S and O leave); O is added up in registers block by block, because a long chain of additions
 // inside the tensor core, which does not round to nearest, would drift (8e-6 at 12k keys).
 // Few tiles over a long context: a cluster of CTAs splits the keys and joins through distributed
 // shared memory. All waits are bounded; TMEM is freed on every path.
@@ -56,13 +56,14 @@ struct TlCfg {
     // or 2 x 224 + 56 = 3 x 168, the launch's)
     static constexpr int kRegsSoftmax = kTiles == 2 ? 112 : kPerSm == 2 ? 104 : 224, kRegsOther = kTiles == 2 || kPerSm == 2 ? 32 : 56;
     static constexpr int kPart = 128 * HDP * 2;              // one tile's Q (one part of it)
-    static constexpr int kParts = SPLIT ? 2 : 1;
+    static constexpr bool kLowTmem = SPLIT && HDP == 256;    // Q's low part in tensor memory, behind S and O
+    static constexpr int kParts = SPLIT && !kLowTmem ? 2 : 1;  // of Q in shared memory
     static constexpr int kQ = kTiles * kParts * kPart;
     static constexpr int kStage = kTlBlk * HDP * 2;          // one K or V block
     static constexpr int kStages = kPerSm == 2 ? (HDP == 64 ? 5 : 2) : HDP == 64 ? 8 : HDP == 256 ? 2 : SPLIT ? 3 : 5;
     static constexpr int kData = kQ + kStages * kStage;
     static_assert(kData >= kRows * HDP * 4 + kTlMaxCluster * kRows * 4, "the joined O and its weights overlay Q and the ring");
-    static_assert(!SPLIT || TILES == 2, "Q's two parts leave too little room for a ring");
+    static_assert(!SPLIT || TILES == 2 || HDP == 256, "Q's two parts leave too little room for a ring");
 };
 template <int HDP, bool SPLIT, int TILES>
 struct TlSmem {
@@ -193,7 +194,33 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
                 return reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + tk) * p.ld_q +
                        (uint64_t)(kvh * p.group + rr - tk * p.group) * p.hd;
             };
-            if constexpr (kSplit) {
+            if constexpr (kSplit && HDP == 256) {  // a row a step; the low parts go to tensor memory below
+#pragma unroll 4
+                for (uint32_t k = 0; k < 16; k++) {
+                    const uint32_t i = w8 * 16 + k;
+                    const bool in = 128 * t + i < n_rows;
+                    const T *src = source(i);
+                    float4 x[2];
+                    float mx = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t c4 = lane + 32 * u;
+                        x[u] = in && 4 * c4 < p.hd ? *reinterpret_cast<const float4 *>(src + 4 * c4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w))));
+                    }
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                    const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255), 2), 252) - 127;
+                    const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
+                    if (lane == 0) sm.mx[0][128 * t + i] = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t c4 = lane + 32 * u, c = c4 >> 1;
+                        *reinterpret_cast<uint2 *>(q + (c >> 3) * (128 * 128) + i * 128 + (((c & 7) ^ (i & 7)) << 4) + 8 * (c4 & 1)) =
+                            make_uint2(pack2<E>(x[u].x * scale, x[u].y * scale), pack2<E>(x[u].z * scale, x[u].w * scale));
+                    }
+                }
+            } else if constexpr (kSplit) {
                 constexpr int kLanes = HDP / 4, kPer = 32 / kLanes;  // lanes of a row (4 values each), rows a warp and step
                 const uint32_t c4 = lane % kLanes, sub = lane / kLanes;
 #pragma unroll
@@ -335,6 +362,10 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
         // work, not between a tile's P and its products (the time is the same while the copies are
         // ahead; a late copy then delays one tile and not both).
         constexpr bool kEarlyV = C::kStages >= 3, kEarlyK = C::kStages >= 4;
+        if constexpr (C::kLowTmem) {
+            named_bar_sync(11, 288);
+            tc_fence_after();
+        }
         if (n_blk > 0) wait(&sm.full[sk], pk);
         for (int32_t j = 0; j <= n_blk; j++) {
             const bool last = j == n_blk;
@@ -370,7 +401,8 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
 #pragma unroll
                             for (int kk = 0; kk < HDP / 16; kk++) {
                                 const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-                                tl_mma_ss(ts, q + (C::kPart >> 4) + off, k + off, kIdS, kk > 0);
+                                if constexpr (C::kLowTmem) tl_mma_ts(ts, tm + 384 + 8 * kk, k + off, kIdS, kk > 0);
+                                else tl_mma_ss(ts, q + (C::kPart >> 4) + off, k + off, kIdS, kk > 0);
                             }
                         }
 #pragma unroll
@@ -422,6 +454,29 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
         if constexpr (kSplit) {
             unscale = t < n_tiles ? sm.mx[0][tr] : 1.0f;
             named_bar_sync(pair, 64);  // both have read it before either writes a maximum there
+        }
+        if constexpr (C::kLowTmem) {  // this thread's half of its row of q once more: what the high part leaves
+            const float scale = 1.0f / unscale;  // a power of two
+            const uint32_t rr = row0 + min(tr, n_rows - 1);
+            const T *src = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + tok) * p.ld_q +
+                           (uint64_t)(kvh * p.group + rr - tok * p.group) * p.hd;
+#pragma unroll 2
+            for (uint32_t c = 0; c < 8; c++) {
+                uint32_t w[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; u++) {
+                    const uint32_t d = 128 * h + 16 * c + 4 * u;
+                    const float4 x = live && d < p.hd ? *reinterpret_cast<const float4 *>(src + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    const float2 a = make_float2(x.x * scale, x.y * scale), b = make_float2(x.z * scale, x.w * scale);
+                    const float2 ah = unpack2<E>(pack2<E>(a.x, a.y)), bh = unpack2<E>(pack2<E>(b.x, b.y));
+                    w[2 * u] = pack2<E>(a.x - ah.x, a.y - ah.y);
+                    w[2 * u + 1] = pack2<E>(b.x - bh.x, b.y - bh.y);
+                }
+                tl_tmem_st8(tmem + 384 + 64 * h + 8 * c + lanes, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            named_bar_sync(11, 288);
         }
         const float cs = p.softcap > 0.0f ? 1.0f : unscale * kLog2e;
         float m = -INFINITY, l = 0.0f;  // m in units of log2, as last rescaled to
@@ -602,16 +657,18 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
                 tc_fence_before();
                 named_bar_sync(9 + t, 256);
                 constexpr int kLanes = kVec < 32 ? kVec : 32, kRows = 32 / kLanes;
-                const uint32_t ch = lane % kLanes;
 #pragma unroll 4
                 for (uint32_t k = 0; k < 16 / kRows; k++) {
                     const uint32_t i = ((sw & 7) * (16 / kRows) + k) * kRows + lane / kLanes;
-                    if (128 * t + i >= n_rows || ch * kPer >= p.hd) continue;
+                    if (128 * t + i >= n_rows) continue;
                     const uint32_t rr = row0 + 128 * t + i;
                     const uint32_t tk = div_group(p, rr);
                     T *orow = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + tk) * p.ld_out +
                               (uint64_t)(kvh * p.group + rr - tk * p.group) * p.hd;
-                    *reinterpret_cast<uint4 *>(orow + ch * kPer) = *reinterpret_cast<const uint4 *>(st + i * kRowB + ((ch ^ (i & 7)) << 4));
+#pragma unroll
+                    for (uint32_t ch = lane % kLanes; ch < (uint32_t)kVec; ch += kLanes)
+                        if (ch * kPer < p.hd)
+                            *reinterpret_cast<uint4 *>(orow + ch * kPer) = *reinterpret_cast<const uint4 *>(st + i * kRowB + ((ch ^ (i & 7)) << 4));
                 }
                 uint32_t bad = __ballot_sync(0xffffffffu, live && chk != 0.0f);
                 named_bar_sync(9 + t, 256);  // every row is written: now the ones that are not finite again
@@ -714,8 +771,6 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
 }
 
 // ---- host ---------------------------------------------------------------------------------------
-bool attention_tile_ok(uint64_t hd, int q_type) { return hd <= 128 || q_type != T_F32; }
-
 // How many CTAs share a tile's keys, by the time that the launch takes in blocks of keys (about 1.8 us
 // each): a CTA's share of the blocks and, for its start and end, 5 more (7 with the join). Two CTAs on
 // an SM hide a part of those (3.5 and 6), but bring each block in twice and take 9 % longer. A launch
@@ -772,18 +827,22 @@ static int launch_tile(rcu_ctx *ctx, const SeqKvMaps &m, SeqAttnParams p, uint32
     return launch_cluster_k<k_attn_tile<T, E, HDP, TILES>>(ctx, (uint32_t)grid, C::kThreads, smem, splits, m.k, m.v, p);
 }
 
-// The form with the smaller cost. f32 queries and head_dim above 128 have one form each: their Q or O
-// leaves no room for the other.
+// The form with the smaller cost. head_dim above 128 has one tile a CTA, f32 queries below have two:
+// O, or Q's two parts, leave no room for the other form.
 template <typename T, typename E, int HDP>
 static int launch_tile_form(rcu_ctx *ctx, const SeqKvMaps &m, const SeqAttnParams &p, uint64_t max_len) {
-    TlPlan one{1, 1.0}, two{1, 0.0};
-    if constexpr (HDP < 256)
-        if (int st = plan_tile<T, E, HDP, 2>(ctx, p, max_len, &two)) return st;
-    if constexpr (!std::is_same<T, float>::value) {
+    TlPlan one, two;
+    if constexpr (HDP == 256) {
         if (int st = plan_tile<T, E, HDP, 1>(ctx, p, max_len, &one)) return st;
-        if (HDP == 256 || one.cost < two.cost) return launch_tile<T, E, HDP, 1>(ctx, m, p, one.splits);
+        return launch_tile<T, E, HDP, 1>(ctx, m, p, one.splits);
+    } else {
+        if (int st = plan_tile<T, E, HDP, 2>(ctx, p, max_len, &two)) return st;
+        if constexpr (!std::is_same<T, float>::value) {
+            if (int st = plan_tile<T, E, HDP, 1>(ctx, p, max_len, &one)) return st;
+            if (one.cost < two.cost) return launch_tile<T, E, HDP, 1>(ctx, m, p, one.splits);
+        }
+        return launch_tile<T, E, HDP, 2>(ctx, m, p, two.splits);
     }
-    if constexpr (HDP < 256) return launch_tile<T, E, HDP, 2>(ctx, m, p, two.splits);
 }
 
 template <typename T, typename E>
@@ -792,8 +851,7 @@ static int launch_tile_hd(rcu_ctx *ctx, SeqAttnParams &p, const SeqKvDesc &kv, u
     const SeqKvMaps *m;
     if (int st = seq_pick_maps(ctx, p, kv, kSeqTileBox, kv.tile, &room, &m)) return st;
     if (p.hd <= 64) return launch_tile_form<T, E, 64>(ctx, *m, p, max_len);
-    if constexpr (!std::is_same<T, float>::value)
-        if (p.hd > 128) return launch_tile_form<T, E, 256>(ctx, *m, p, max_len);
+    if (p.hd > 128) return launch_tile_form<T, E, 256>(ctx, *m, p, max_len);
     return launch_tile_form<T, E, 128>(ctx, *m, p, max_len);
 }
 

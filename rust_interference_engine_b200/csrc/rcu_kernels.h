@@ -131,12 +131,10 @@ struct SeqKvDesc {
 // (max_new too: 0 when unknown). q_type T_F32 or T_F16 over f16, or T_BF16 over bf16.
 int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len,
                          uint64_t max_new);
-// Its kernel for sequences of many query rows per KV head (rcu_attn_tile.cu), f32 queries up to
-// head_dim 128.
+// Its kernel for sequences of many query rows per KV head (rcu_attn_tile.cu).
 // From this many rows on it is the faster one (f16, 16,000 keys: 31 against 36 us at 32 rows, 46
 // against 36 at 64; f32: 57 against 55 and 98 against 56).
 constexpr uint32_t kTileMinRows = 40;
-bool attention_tile_ok(uint64_t hd, int q_type);
 constexpr uint32_t kSeqFewBox = 16, kSeqTileBox = 128;  // rows of a load: kSeqFewBox; a page's, kSeqTileBox at most
 int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len);
 // log p of targets, entropy and the largest top_k of rows of logits (rcu_logprobs.cu).

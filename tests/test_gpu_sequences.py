@@ -462,3 +462,25 @@ def test_wide_heads_in_chunks(env, hd, window):
     c.check(c.run(window), window)
     c = Case(*env, [(100, 300), (1, 50), (33, 33)], 6, 2, hd, 16, "f16", seed=28)
     c.check(c.run(window, 20.0), window, 20.0)
+
+
+@pytest.mark.parametrize("hd", [160, 224, 256])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (700, 0.0), (0, 20.0)])
+def test_wide_heads_of_f32_queries(env, hd, window, softcap):
+    """f32 queries of head_dim above 128 in chunks: keys split over a cluster or not, rows that are part of a tile."""
+    for seqs, n_head, n_kv, ps, seed in (([(60, 3000)], 4, 1, 64, 31), ([(100, 300), (1, 50), (33, 33)], 6, 2, 16, 32),
+                                         ([(11, 5000)], 16, 4, 16, 33), ([(150, 150)] * 4, 8, 8, 128, 34)):
+        c = Case(*env, seqs, n_head, n_kv, hd, ps, "f32", seed=seed)
+        c.check(c.run(window, softcap), window, softcap)
+
+
+def test_a_nan_query_of_a_wide_head_stays_in_its_row(env):
+    torch = env[0]
+    c = Case(*env, [(80, 200)], 4, 1, 256, 16, "f32", seed=35)
+    out = c.run()
+    c.q[40, :256] = float("nan")
+    got = c.run()
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[40, :256] = False
+    assert got[40, :256].isnan().all()
+    assert torch.equal(got[keep], out[keep])
