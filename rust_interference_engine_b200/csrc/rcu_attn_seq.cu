@@ -466,7 +466,10 @@ int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const
     // tokens in a launch of their own).
     const uint64_t new_max = max_new ? max_new : p.b.n_tok <= p.b.n_seq ? 1 : p.b.n_tok;
     const uint64_t most = std::min<uint64_t>(new_max, p.b.n_tok) * p.group;
-    if (most < kTileMinRows) return launch_attention_few(ctx, p, q_type, kv, max_len, most);
+    // Above kSqMaxRows rows k_attn_seq reads keys and values more than once, which costs most where the
+    // sequences fill the device.
+    const bool full = most > kSqMaxRows && p.b.n_seq * p.n_kv >= kTileMinPairs;
+    if (most < kTileMinRows && !full) return launch_attention_few(ctx, p, q_type, kv, max_len, most);
     return launch_attention_tile(ctx, p, q_type, kv, max_len);
 }
 

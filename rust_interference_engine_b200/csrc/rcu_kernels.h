@@ -135,6 +135,10 @@ int launch_seq_attention(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const
 // From this many rows on it is the faster one (f16, 16,000 keys: 31 against 36 us at 32 rows, 46
 // against 36 at 64; f32: 57 against 55 and 98 against 56).
 constexpr uint32_t kTileMinRows = 40;
+// From 17 rows on where sequences times KV heads are at least this many (20 rows, 16 sequences of 2000
+// to 4000 keys, 4 KV heads, f16: 29 against 43 us; 32 rows, 8 sequences: 21 against 21; 17 rows, 48
+// sequences, one KV head: 33 against 27).
+constexpr uint32_t kTileMinPairs = 64;
 constexpr uint32_t kSeqFewBox = 16, kSeqTileBox = 128;  // rows of a load: kSeqFewBox; a page's, kSeqTileBox at most
 int launch_attention_tile(rcu_ctx *ctx, const SeqAttnParams &p, int q_type, const SeqKvDesc &kv, uint64_t max_len);
 // log p of targets, entropy and the largest top_k of rows of logits (rcu_logprobs.cu).

@@ -484,3 +484,11 @@ def test_a_nan_query_of_a_wide_head_stays_in_its_row(env):
     keep[40, :256] = False
     assert got[40, :256].isnan().all()
     assert torch.equal(got[keep], out[keep])
+
+
+@pytest.mark.parametrize("hd,ty", [(64, "f16"), (128, "f32"), (256, "f32")])
+def test_single_tokens_of_large_groups(env, hd, ty):
+    """17 to 39 query rows a KV head: enough sequences to fill the device, and few."""
+    for n, seed in ((64, 36), (3, 37)):
+        c = Case(*env, [(1, 1 + 17 * i % 300) for i in range(n)] + [(0, 5)], 20, 1, hd, 32, ty, seed=seed)
+        c.check(c.run())
