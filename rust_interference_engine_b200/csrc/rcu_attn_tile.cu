@@ -532,11 +532,10 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
                 }
             }
             sm.mx[h][tr] = mx;
-            named_bar_sync(pair, 64);
-            mx = max3_nan(mx, sm.mx[h ^ 1][tr], -INFINITY) * cs;
-            const bool grow = kSplit ? mx > m : mx > m + kTlLazy || (m == -INFINITY && mx > m);
             if constexpr (kSplit) {
-                if (j > jb[t]) {  // add the last block's P V
+                // Add the last block's P V, before the pair's barrier: the next P V starts when the first
+                // half's P is there and writes all of O's columns, the other half's among them.
+                if (j > jb[t]) {
 #pragma unroll
                     for (int c = 0; c < HDP / 16; c++) {
                         uint32_t v[8];
@@ -545,8 +544,13 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
 #pragma unroll
                         for (int i = 0; i < 8; i++) o[8 * c + i] += __uint_as_float(v[i]);
                     }
+                    tc_fence_before();
                 }
             }
+            named_bar_sync(pair, 64);
+            if constexpr (kSplit) tc_fence_after();
+            mx = max3_nan(mx, sm.mx[h ^ 1][tr], -INFINITY) * cs;
+            const bool grow = kSplit ? mx > m : mx > m + kTlLazy || (m == -INFINITY && mx > m);
             if (__any_sync(0xffffffffu, grow)) {  // the same for the other warp of these rows
                 const float mn = grow ? mx : m;
                 const float a = mn == m ? 1.0f : ex2(m - mn);

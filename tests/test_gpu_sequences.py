@@ -492,3 +492,35 @@ def test_single_tokens_of_large_groups(env, hd, ty):
     for n, seed in ((64, 36), (3, 37)):
         c = Case(*env, [(1, 1 + 17 * i % 300) for i in range(n)] + [(0, 5)], 20, 1, hd, 32, ty, seed=seed)
         c.check(c.run())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("seqs,n_kv", [([(300, 2300)], 4), ([(40, 6000)], 2), ([(200, 900), (130, 1400)] * 8, 8)])
+def test_f32_chunks_have_the_same_bits_every_time(env, hd, seqs, n_kv):
+    """A tile's O is read back block by block while the tensor core goes on: whichever warp is late,
+    the sums are the same. One tile a CTA and two, keys split over a cluster and whole."""
+    torch, rie, ctx = env
+    g = torch.Generator(device="cuda").manual_seed(38)
+    n_head, ps = 2 * n_kv, 32
+    need = [-(-n // ps) for _, n in seqs]
+    pages = torch.zeros(len(seqs), max(need), dtype=torch.int32, device="cuda")
+    for i, n in enumerate(need):
+        pages[i, :n] = torch.arange(sum(need[:i]), sum(need[:i]) + n, dtype=torch.int32)
+    cache_k, cache_v = (torch.randn(sum(need), n_kv, ps, hd, generator=g, device="cuda").half() for _ in "kv")
+    cache = rie.PagedCache(ctx, n_kv, hd, ps, sum(need), k=cache_k, v=cache_v)
+    n_tok = sum(n for n, _ in seqs)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum([n for n, _ in seqs])]), dtype=torch.int32, device="cuda")
+    batch = rie.SeqBatch(cu, torch.tensor([n for _, n in seqs], dtype=torch.int32, device="cuda"), pages, n_tok)
+    q = torch.randn(n_tok, n_head * hd, generator=g, device="cuda") * (2 / np.sqrt(hd))
+    first, again = torch.zeros_like(q), torch.zeros_like(q)
+    rie.paged_attention(ctx, cache, batch, q, n_head, first)
+    for _ in range(40):
+        again.zero_()
+        rie.paged_attention(ctx, cache, batch, q, n_head, again)
+        ctx.sync()
+        assert torch.equal(first, again)
+    i, (new, length) = len(seqs) - 1, seqs[-1]
+    ks, vs = (x[pages[i, :need[i]].long()].transpose(1, 2).reshape(-1, n_kv, hd)[:length].double().cpu().numpy() for x in (cache_k, cache_v))
+    a = n_tok - new
+    check_rows(first[a:a + 3].double().cpu().numpy(), q[a:a + 3].double().cpu().numpy(), [ks[:length - new + 3]], [vs[:length - new + 3]],
+               [(0, 3, length - new + 3)], n_head, n_kv, hd, 0, 0.0, "f32")
