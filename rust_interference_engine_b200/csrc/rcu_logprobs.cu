@@ -34,6 +34,9 @@ constexpr int kLpGroups = 256;                   // groups whose maxima give a b
 constexpr int kLpKeep = kLpCap / 2;
 
 constexpr int kLpStages = 2;
+// exp(d) is 0 in f32 from here on down. Farther distances (-inf; masks of the type's lowest value,
+// whose products with d leave f32's range) are taken for this one, so that 0 * d stays 0.
+constexpr float kLpFar = -1000.0f;
 
 struct LpSmem {
     uint64_t full[kLpStages], empty[kLpStages];
@@ -66,19 +69,19 @@ struct LpSum {
             return;
         }
         const float d = m - mn, a = ex2(d * kLog2e);
-        w = a * fmaf(d, z, w);
+        w = a * fmaf(fmaxf(d, kLpFar), z, w);  // where a is 0, d z may be past the largest number; a NaN stays in z
         z *= a;
         m = mn;
     }
-    // 16 values, none above m; low: one of them is -inf, which adds nothing
-    __device__ __forceinline__ void add16(const float (&f)[16], bool low) {
+    // 16 values, none above m; far: one of them is kLpFar or more below m and adds nothing
+    __device__ __forceinline__ void add16(const float (&f)[16], bool far) {
         const float2 nm = make_float2(-m, -m), c = make_float2(kLog2e, kLog2e);
         float2 z2[2] = {}, w2[2] = {};
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             float2 d = add2(make_float2(f[2 * i], f[2 * i + 1]), nm);
             const float2 y = mul2(d, c), e = make_float2(ex2(y.x), ex2(y.y));
-            if (low) d.x = fmaxf(d.x, -1000.0f), d.y = fmaxf(d.y, -1000.0f);  // a NaN stays in e
+            if (far) d.x = fmaxf(d.x, kLpFar), d.y = fmaxf(d.y, kLpFar);  // a NaN stays in e
             z2[i & 1] = add2(z2[i & 1], e);
             w2[i & 1] = fma2(e, d, w2[i & 1]);
         }
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) k_logprobs(co
         if (top > a.m) a.raise(top);
         if (top != top) a.z = top;
         if (a.m != -INFINITY) {
-            if (low == -INFINITY) a.add16(f, true);
+            if (low - a.m < kLpFar) a.add16(f, true);
             else a.add16(f, false);
         }
         if (k == 0) continue;

@@ -100,6 +100,45 @@ def test_orders_that_defeat_the_bound(env, k, kind):
     check(x, targets, k, run(env, torch.from_numpy(x.copy()).cuda(), targets, k), n)
 
 
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("value", ["lowest", -1e38, -3e37, -1e34, -2e3])
+@pytest.mark.parametrize("k", [0, 3])
+def test_masks_of_very_low_values(env, ty, value, k):
+    """Tokens masked by a finite value, in runs that fill a thread's, a warp's and a CTA's values, and
+    rows that are all of it: the entropy is that of the other tokens."""
+    torch = env[0]
+    t = {"f32": torch.float32, "bf16": torch.bfloat16}[ty]
+    n, low = 60001, torch.finfo(t).min if value == "lowest" else value
+    x = torch.from_numpy(np.random.default_rng(3).standard_normal((7, n)) * 4)
+    keep = torch.zeros(7, n, dtype=torch.bool)
+    keep[0, n // 2:] = True
+    keep[1, :n // 2] = True
+    keep[2, [5, 777, 30000, 59999]] = True
+    keep[3] = True
+    keep[3, 20000:26000] = False
+    keep[4, n - 1] = True
+    keep[5, ::16] = True  # row 6: nothing but the mask
+    x = torch.where(keep, x, torch.tensor(float(low), dtype=torch.float64)).to(t).cuda()
+    xn = x.double().cpu().numpy()
+    targets = np.array([n - 1, 0, 777, 21000, n - 1, 16, 9])
+    for rows in (slice(0, 7), slice(0, 4), slice(4, 7)):
+        check(xn[rows], targets[rows], k, run(env, x[rows], targets[rows], k), n)
+
+
+@pytest.mark.parametrize("rows", [2, 9])
+def test_rows_that_span_more_than_the_largest_number(env, rows):
+    """Finite logits whose distance from the maximum has no f32 value: they add nothing."""
+    torch = env[0]
+    x = np.full((rows, 20000), -3e38, dtype=np.float32)
+    x[:, 3::5] = np.random.default_rng(4).standard_normal((rows, 4000))
+    x[:, 100:200] = 3e38
+    got = run(env, torch.from_numpy(x).cuda(), np.full(rows, 150), 100)
+    want = np.log(100.0)  # of 100 equal values; ln z rounds once, a sum of 100 ones is exact
+    assert (np.abs(got["entropy"] - want) <= 2.0 ** -22 * want).all()
+    assert (np.abs(got["logprob"] + want) <= 2.0 ** -22 * want).all()
+    assert (got["top_ids"] == np.arange(100, 200)).all()
+
+
 def test_rows_without_a_distribution(env):
     torch, rie, ctx = env
     n = 5000
