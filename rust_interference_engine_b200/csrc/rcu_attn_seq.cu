@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
         float L, M;
         float acc[HDP / 32] = {};
         if (p.splits == 1) {
-            L = sm.cl[r];
+            L = sm.cl[r], M = sm.cm[r];
             for (int i = 0; i < HDP / 32; i++) acc[i] = oc[r * S::kLd + lane + 32 * i];
         } else {
             const uint32_t am = smem_u32(&sm.cm[r]), al2 = smem_u32(&sm.cl[r]), ao = smem_u32(oc + r * S::kLd + lane);
@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(kSqWarps * 32) k_attn_seq(const __grid_constan
             fine = fine && (isfinite(v) || d >= p.hd);
             if (d < p.hd) orow[d] = from_f32<T>(v);
         }
-        if (!__all_sync(0xffffffffu, fine)) {
+        if (!__all_sync(0xffffffffu, fine) && !seq_row_settled<T>(M, L)) {
             __syncwarp();
-            seq_attn_row<T, E>(p, sp, t, kvh, gq);
+            seq_attn_row<T, E, HDP>(p, sp, t, kvh, gq);
         }
     }
     if (p.splits > 1) cluster_sync_all();  // no CTA leaves while another reads its shared memory

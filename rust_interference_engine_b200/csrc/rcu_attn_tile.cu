@@ -674,13 +674,16 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
                         if (ch * kPer < p.hd)
                             *reinterpret_cast<uint4 *>(orow + ch * kPer) = *reinterpret_cast<const uint4 *>(st + i * kRowB + ((ch ^ (i & 7)) << 4));
                 }
-                uint32_t bad = __ballot_sync(0xffffffffu, live && chk != 0.0f);
+                uint32_t bad = __ballot_sync(0xffffffffu, live && chk != 0.0f && !seq_row_settled<T>(m, l));
+                if (lane == 0) sm.mx[h][128 * t + 32 * (warp & 3)] = __uint_as_float(bad);
                 named_bar_sync(9 + t, 256);  // every row is written: now the ones that are not finite again
+                bad |= __float_as_uint(sm.mx[h ^ 1][128 * t + 32 * (warp & 3)]);
+                bad &= h ? 0xaaaaaaaau : 0x55555555u;  // shared by the two warps of these rows
                 while (bad) {
                     const int b = __ffs((int)bad) - 1;
                     bad &= bad - 1;
                     const uint32_t rr = row0 + 128 * t + 32 * (warp & 3) + b;
-                    seq_attn_row<T, E>(p, sp, div_group(p, rr), kvh, rr - div_group(p, rr) * p.group);
+                    seq_attn_row<T, E, HDP>(p, sp, div_group(p, rr), kvh, rr - div_group(p, rr) * p.group);
                 }
             }
             tc_fence_before();
@@ -704,6 +707,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
         tc_fence_before();
         cluster_sync_all();
         // weight of each CTA's part of row i: 2^(m_c - max m) / sum_c l_c 2^(m_c - max m)
+        constexpr uint32_t kSettled = 0x7ffffffeu;  // a NaN
         float *wt = reinterpret_cast<float *>(sm.data + kTlRows * HDP * 4);
         if (threadIdx.x - 32 * kSoft0 < n_rows) {
             const uint32_t i = threadIdx.x - 32 * kSoft0, am = smem_u32(&sm.mx[0][i]), al = smem_u32(&sm.mx[1][i]);
@@ -723,7 +727,8 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
 #pragma unroll
             for (int c = 0; c < kTlMaxCluster; c++)
                 if (c < (int)p.splits) wt[c * kTlRows + i] = mc[c] * inv;
-            if (!isfinite(inv)) wt[i] = __uint_as_float(0x7fffffffu);  // no keys, or a NaN: the row is made again
+            // no keys, or a NaN: the row is made again, unless NaN is its answer
+            if (!isfinite(inv)) wt[i] = __uint_as_float(seq_row_settled<T>(M, L) ? kSettled : 0x7fffffffu);
         }
         named_bar_sync(15, kTlSoftWarps * 32);
         constexpr int kVec = HDP / 4, kLn = kVec < 32 ? kVec : 32, kPerRow = kVec / kLn;  // 16-byte chunks of a row, lanes, chunks a lane
@@ -751,6 +756,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
                 if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(orow + 4 * ch) = v;
                 else *reinterpret_cast<uint2 *>(orow + 4 * ch) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
             }
+            if (in && __float_as_uint(wt[i]) == kSettled) fine = true;
             uint32_t bad = __ballot_sync(0xffffffffu, !fine);
             if (bad) {
                 __syncwarp();
@@ -758,7 +764,7 @@ __global__ void __launch_bounds__(TlCfg<HDP, std::is_same<T, float>::value, TILE
                 for (int r = 0; r < 32 / kLn; r++)
                     if (bad >> (r * kLn) & (kLn == 32 ? 0xffffffffu : (1u << kLn) - 1)) {
                         const uint32_t rb = __shfl_sync(0xffffffffu, rr, r * kLn);
-                        seq_attn_row<T, E>(p, sp, div_group(p, rb), kvh, rb - div_group(p, rb) * p.group);
+                        seq_attn_row<T, E, HDP>(p, sp, div_group(p, rb), kvh, rb - div_group(p, rb) * p.group);
                     }
             }
         }

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "rcu_kernels.h"
 #include "rcu_tc.cuh"
@@ -272,50 +273,111 @@ inline void set_group(SeqAttnParams &p, uint32_t group) {
 // One output row by one warp, from the formula, over the attended keys alone. The tiled kernels
 // multiply the probability 0 of a masked key with its value, which is NaN where that value is an
 // infinity or NaN; a row that comes out not finite is made again here, where masked keys are not
-// touched. An attended NaN or infinity stays what the formula makes of it.
-template <typename T, typename E>
+// touched. An attended NaN or infinity stays what the formula makes of it. 32 keys a step, four at a
+// time: eight lanes take a key, each the 16-byte pieces sub, sub + 8, .. of its row. A row of its own on
+// an SM is bound by the latency of its loads (0.16 us a key; taken one a step it was 2.4 us), the
+// rows of a tile by the instructions (512 tokens over 12,800 keys, 32 heads, a tile in which every row
+// is made again: 14 ms against 175). Unrolled further or with the next rows fetched ahead it was slower.
+template <typename T, typename E, int HDP>
 __device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan &sp, uint32_t t, uint32_t kvh, uint32_t g) {
-    const uint32_t lane = threadIdx.x & 31, head = kvh * p.group + g;
+    constexpr int NC = HDP / 64;
+    const uint32_t lane = threadIdx.x & 31, sub = lane & 7, grp = lane >> 3, pieces = p.hd / 8, head = kvh * p.group + g;
     const int32_t pos = sp.pos(t), lo = p.window > 0 ? max(pos - (int32_t)p.window + 1, 0) : 0;
     const T *q = reinterpret_cast<const T *>(p.q) + (uint64_t)(sp.first + t) * p.ld_q + (uint64_t)head * p.hd;
     T *out = reinterpret_cast<T *>(p.out) + (uint64_t)(sp.first + t) * p.ld_out + (uint64_t)head * p.hd;
     const uint32_t kvo = p.b.pages ? 0u : kvh * (uint32_t)p.head_kv;
-    float qv[8], o[8];
+    float qv[NC][8], o[NC][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t d = lane + 32 * i;
-        qv[i] = d < p.hd ? to_f32(q[d]) : 0.0f;
-        o[i] = 0.0f;
-    }
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            qv[c][i] = sub + 8 * c < pieces ? to_f32(q[8 * (sub + 8 * c) + i]) : 0.0f;
+            o[c][i] = 0.0f;
+        }
+    // this lane's pieces of row r of x; loads without a branch, so that several are in flight
+    auto fetch = [&](const void *x, uint32_t r, uint4 (&u)[NC]) {
+        const E *src = reinterpret_cast<const E *>(x) + (uint64_t)(r == kNoRow ? 0 : r) * p.ld_kv + kvo;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            u[c] = __ldg(reinterpret_cast<const uint4 *>(src + 8 * min(sub + 8 * c, pieces - 1)));
+            if (r == kNoRow || sub + 8 * c >= pieces) u[c] = make_uint4(0, 0, 0, 0);
+        }
+    };
+    // the group's keys are 4 i + grp, i = 0 .. 7; lane `sub` of it holds key i = sub's row and score
+    auto place = [&](int64_t j0) { return j0 + 4 * sub + grp <= pos ? seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)j0 + 4 * sub + grp) : kNoRow; };
     float m = -INFINITY, l = 0.0f;
-    for (int64_t j = lo; j <= pos; j++) {  // pos may be 2^31 - 1
-        const uint32_t row = seq_kv_row(p.b, sp, p.n_kv, kvh, (uint32_t)j);
-        const E *kr = reinterpret_cast<const E *>(p.k) + (uint64_t)row * p.ld_kv + kvo;
-        const E *vr = reinterpret_cast<const E *>(p.v) + (uint64_t)row * p.ld_kv + kvo;
-        float s = 0.0f;
+    uint32_t next = place(lo);
+    for (int64_t j0 = lo; j0 <= pos; j0 += 32) {  // pos may be 2^31 - 1
+        const bool in = j0 + 4 * sub + grp <= pos;
+        const uint32_t row = next;
+        next = place(j0 + 32);
+        float s = -INFINITY;
+#pragma unroll 4
+        for (uint32_t i = 0; i < 8; i++) {
+            uint4 u[NC];
+            fetch(p.k, __shfl_sync(0xffffffffu, row, (lane & 24) | i), u);
+            float x = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t d = lane + 32 * i;
-            if (d < p.hd && row != kNoRow) s = fmaf(qv[i], to_f32(kr[d]), s);
+            for (int c = 0; c < NC; c++) {
+                const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float2 f = unpack2<E>(w[k]);
+                    x = fmaf(qv[c][2 * k + 1], f.y, fmaf(qv[c][2 * k], f.x, x));
+                }
+            }
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+            if (sub == i && in) s = x;
         }
+        if (p.softcap > 0.0f && in) s = p.softcap * tanhf(s / p.softcap);
+        float mn = fmaxf(m, s);  // leaves a NaN out
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (p.softcap > 0.0f) s = p.softcap * tanhf(s / p.softcap);
-        const float mn = s > m ? s : m;
-        const float a = m == mn ? 1.0f : expf(m - mn), e = s == -INFINITY && mn == -INFINITY ? 0.0f : expf(s - mn);
+        for (int d = 16; d > 0; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+        const float a = m == mn ? 1.0f : expf(m - mn), e = s == -INFINITY ? 0.0f : expf(s - mn);
+        float sum = e;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         m = mn;
-        l = l * a + e;
+        l = l * a + sum;
+        if (l != l) break;  // a score is NaN or +inf: so is the row, whatever follows
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t d = lane + 32 * i;
-            if (d < p.hd) o[i] = o[i] * a + e * (row != kNoRow ? to_f32(vr[d]) : 0.0f);
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[c][i] *= a;
+#pragma unroll 4
+        for (uint32_t i = 0; i < 8; i++) {
+            const float ei = __shfl_sync(0xffffffffu, e, (lane & 24) | i);
+            uint4 u[NC];
+            fetch(p.v, __shfl_sync(0xffffffffu, row, (lane & 24) | i), u);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const uint32_t w[4] = {u[c].x, u[c].y, u[c].z, u[c].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float2 f = unpack2<E>(w[k]);
+                    o[c][2 * k] = fmaf(ei, f.x, o[c][2 * k]);
+                    o[c][2 * k + 1] = fmaf(ei, f.y, o[c][2 * k + 1]);
+                }
+            }
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t d = lane + 32 * i;
-        if (d < p.hd) out[d] = from_f32<T>(lo > pos ? 0.0f : o[i] / l);
-    }
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            o[c][i] += __shfl_xor_sync(0xffffffffu, o[c][i], 8);
+            o[c][i] += __shfl_xor_sync(0xffffffffu, o[c][i], 16);
+            if (grp == 0 && sub + 8 * c < pieces) out[8 * (sub + 8 * c) + i] = from_f32<T>(lo > pos ? 0.0f : o[c][i] / l);
+        }
+}
+// Whether a row that came out not finite, with the largest score m (in units of log2) and the sum l, is
+// its answer already. A masked score adds 0 to the sum whatever it is, so that a NaN there is from an
+// attended score that is NaN or +inf. Not so where m overflowed; nor for f32 queries, whose two parts
+// make NaN of a score of -inf: those rows are made again.
+template <typename T>
+__device__ __forceinline__ bool seq_row_settled(float m, float l) {
+    return !std::is_same<T, float>::value && l != l && m < INFINITY;
 }
 
 // ---- host ---------------------------------------------------------------------------------------

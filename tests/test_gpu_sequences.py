@@ -524,3 +524,45 @@ def test_f32_chunks_have_the_same_bits_every_time(env, hd, seqs, n_kv):
     a = n_tok - new
     check_rows(first[a:a + 3].double().cpu().numpy(), q[a:a + 3].double().cpu().numpy(), [ks[:length - new + 3]], [vs[:length - new + 3]],
                [(0, 3, length - new + 3)], n_head, n_kv, hd, 0, 0.0, "f32")
+
+
+@pytest.mark.parametrize("ty,times", [("f16", 3), ("f32", 12)])
+@pytest.mark.parametrize("shape", ["decode", "chunk", "packed"])
+def test_a_nan_key_does_not_slow_the_call(env, ty, times, shape):
+    """Rows that attend a NaN key are NaN, and known to be: the formula is not gone through again key by
+    key (some thousand times the call's own time). f32 rows go through it as far as the NaN, which is early here."""
+    torch, rie, ctx = env
+    T, g = dtype(torch, ty), torch.Generator(device="cuda").manual_seed(39)
+    n_head, n_kv, hd, ps = 8, 2, 128, 64
+    new, length = {"decode": (1, 60000), "chunk": (200, 9000), "packed": (3000, 3000)}[shape]
+    n_pages = -(-length // ps)
+    kp, vp = (torch.randn(n_pages, n_kv, ps, hd, generator=g, device="cuda").half() for _ in "kv")
+    cache = rie.PagedCache(ctx, n_kv, hd, ps, n_pages, k=kp, v=vp)
+    cu, ln = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, new], [length]))
+    batch = rie.SeqBatch(cu, ln, torch.arange(n_pages, dtype=torch.int32, device="cuda")[None], new, max_len=length, max_new=new)
+    q = (torch.randn(new, n_head * hd, generator=g, device="cuda") / 8).to(T)
+    k, v = (x.transpose(1, 2).reshape(-1, n_kv * hd)[:length].contiguous() for x in (kp, vp))
+    out = torch.zeros_like(q)
+
+    def call():
+        if shape == "packed":
+            rie.packed_attention(ctx, q, k, v, cu, n_head, n_kv, hd, out, max_len=length)
+        else:
+            rie.paged_attention(ctx, cache, batch, q, n_head, out)
+
+    def time():
+        call()
+        ends = [torch.cuda.Event(enable_timing=True) for _ in range(6)]
+        for e in ends:
+            e.record()
+            call()
+        ctx.sync()
+        return min(a.elapsed_time(b) for a, b in zip(ends, ends[1:]))
+
+    clean = time()
+    assert torch.isfinite(out).all()
+    kp[0, :, 5] = float("nan")
+    k[5] = float("nan")
+    assert time() <= times * clean
+    first = 5 if shape == "packed" else 0
+    assert torch.isfinite(out[:first]).all() and torch.isnan(out[first:]).all()
