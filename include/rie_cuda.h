@@ -194,7 +194,8 @@ RCU_API int32_t rcu_attention(rcu_ctx *ctx, const rcu_kv *kv, const float *q_dev
  * f16 (kv_type RCU_KV_F16; the other formats return RCU_ERR_UNSUPPORTED), head_dim a multiple of
  * 32 up to 256. k_dev / v_dev: the caller's pools of n_pages * n_head_kv * page_size * head_dim
  * f16 each (16-byte aligned, not copied, not freed), or both NULL: the library allocates zeroed
- * ones. Which page belongs to whom is the caller's bookkeeping. */
+ * ones. Which page belongs to whom is the caller's bookkeeping. A pool serves any context of the
+ * device it was made on, and may outlive the one that made it. */
 typedef struct rcu_paged rcu_paged;
 RCU_API int32_t rcu_paged_create(rcu_ctx *ctx, int32_t kv_type, uint64_t n_head_kv, uint64_t head_dim,
                                  uint64_t page_size, uint64_t n_pages, void *k_dev, void *v_dev, rcu_paged **out);

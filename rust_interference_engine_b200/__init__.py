@@ -525,6 +525,8 @@ def paged_attention(ctx: Context, cache: PagedCache, batch: SeqBatch, q, n_head:
                     softcap: float | None = None) -> None:
     """Causal GQA attention of the batch's new tokens over their pages (rcu_paged_attention); q
     (n_tok x n_head*head_dim, f32 or f16) already x attn_scale, out the same type."""
+    if cache.ctx.device != ctx.device:
+        raise ValueError(f"cache: on device {cache.ctx.device}, the context is on {ctx.device}")
     width = n_head * cache.head_dim
     qp, ty, ld = _rows(ctx, q, batch.n_tok, width, "q")
     op, ty_o, ld_o = _rows(ctx, out, batch.n_tok, width, "out")

@@ -153,10 +153,11 @@ struct LogprobParams {
 };
 int launch_logprobs(rcu_ctx *ctx, const LogprobParams &p, int type);
 
-// Makes the context's device the current one for the length of a call.
+// Makes a device (the context's) the current one for the length of a call.
 struct DeviceGuard {
     int prev = -1, dev;
-    explicit DeviceGuard(const rcu_ctx *ctx) : dev(ctx->device) {
+    explicit DeviceGuard(const rcu_ctx *ctx) : DeviceGuard(ctx->device) {}
+    explicit DeviceGuard(int device) : dev(device) {
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
         if (prev != dev) cudaSetDevice(dev);
     }

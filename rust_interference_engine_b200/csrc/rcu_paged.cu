@@ -12,7 +12,7 @@
 #include "rcu_seq.cuh"
 
 struct rcu_paged {
-    rcu_ctx *ctx = nullptr;
+    int device = 0;  // not the context: a pool may outlive the one that made it
     uint64_t n_kv = 0, hd = 0, page_size = 0, n_pages = 0;
     uint32_t page_shift = 0;
     void *k = nullptr, *v = nullptr;
@@ -108,6 +108,7 @@ static int check_batch(rcu_ctx *ctx, uint64_t n_tok, uint64_t n_seq) {
 }
 static int check_seqs(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s, SeqView *v) {
     if (!pg || !s || !s->cu || !s->len || !s->pages) return set_err(ctx, RCU_ERR_INVALID, "null argument");
+    if (ctx && pg->device != ctx->device) return set_err(ctx, RCU_ERR_INVALID, "paged cache: on another device than the context");
     if (int st = check_batch(ctx, s->n_tok, s->n_seq)) return st;
     if (s->ld_pages == 0 || s->ld_pages * pg->page_size > 0x7fffffffull)
         return set_err(ctx, RCU_ERR_INVALID, "page table: 1 .. 2^31 / page_size pages a sequence");
@@ -151,7 +152,7 @@ int32_t rcu_paged_create(rcu_ctx *ctx, int32_t kv_type, uint64_t n_head_kv, uint
     DeviceGuard guard(ctx);
     rcu_paged *pg = new (std::nothrow) rcu_paged();
     if (!pg) return set_err(ctx, RCU_ERR_OOM, "host allocation failed");
-    pg->ctx = ctx;
+    pg->device = ctx->device;
     pg->n_kv = n_head_kv;
     pg->hd = head_dim;
     pg->page_size = page_size;
@@ -186,7 +187,7 @@ int32_t rcu_paged_create(rcu_ctx *ctx, int32_t kv_type, uint64_t n_head_kv, uint
 void rcu_paged_free(rcu_paged *pg) {
     if (!pg) return;
     if (pg->owned) {
-        DeviceGuard guard(pg->ctx);
+        DeviceGuard guard(pg->device);
         cudaFree(pg->k);
         cudaFree(pg->v);
     }

@@ -566,3 +566,27 @@ def test_a_nan_key_does_not_slow_the_call(env, ty, times, shape):
     assert time() <= times * clean
     first = 5 if shape == "packed" else 0
     assert torch.isfinite(out[:first]).all() and torch.isnan(out[first:]).all()
+
+
+def test_a_pool_of_another_device_is_refused(env):
+    """By the C entry points too, before they launch anything; and a pool outlives the context that made it."""
+    import ctypes
+    torch, rie, ctx = env
+    lib = ctx._lib
+    own = rie.Context(0, torch.cuda.current_stream())
+    pool = ctypes.c_void_p()
+    assert lib.rcu_paged_create(own.ptr, 0, 2, 64, 16, 8, None, None, ctypes.byref(pool)) == 0
+    own.sync()
+    own.close()
+    cu, ln, pages = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 1], [3], [[0]]))
+    batch = rie.SeqBatch(cu, ln, pages, 1)
+    q, out = torch.randn(1, 256, device="cuda"), torch.ones(1, 256, device="cuda")
+    assert lib.rcu_paged_attention(ctx.ptr, pool, batch._ref, q.data_ptr(), 0, 256, 4, 0, 0.0, out.data_ptr(), 256) == 0
+    ctx.sync()
+    assert (out == 0).all()  # zeroed pages
+    if torch.cuda.device_count() > 1:
+        other = rie.Context(1)
+        for st in (lib.rcu_paged_attention(other.ptr, pool, batch._ref, q.data_ptr(), 0, 256, 4, 0, 0.0, out.data_ptr(), 256),
+                   lib.rcu_paged_store(other.ptr, pool, batch._ref, q.data_ptr(), q.data_ptr(), 0, 128)):
+            assert st == 1 and b"another device" in lib.rcu_last_error(other.ptr)
+    lib.rcu_paged_free(pool)

@@ -89,3 +89,16 @@ def test_seq_batch_checks_its_tensors():
         rie.SeqBatch(cu.long(), cu[:2].clone(), torch.zeros(2, 4, dtype=torch.int32), 1)
     with pytest.raises(ValueError, match="2-dimensional"):
         rie.SeqBatch(cu, cu[:2].clone(), cu, 1)
+
+
+def test_a_cache_of_another_device_is_refused():
+    """Before anything of it is used."""
+    import rust_interference_engine_b200 as rie
+
+    class At:
+        def __init__(self, **kw):
+            self.__dict__.update(kw)
+
+    cache = At(ctx=At(device=0), head_dim=64, ptr=None)
+    with pytest.raises(ValueError, match="cache: on device 0, the context is on 1"):
+        rie.paged_attention(At(device=1), cache, At(n_tok=1), None, 1, None)
