@@ -205,8 +205,8 @@ RCU_API int32_t rcu_paged_device_ptrs(const rcu_paged *pg, void **k_dev, void **
  * kernels run, so a captured graph replays with what they hold then; n_tok, n_seq and ld_pages
  * are fixed by the capture. What the kernels find out of range there (offsets that fall or leave
  * the batch, a len below the sequence's new tokens or above its table, a page number outside the
- * pool) they skip, read as zeros or clamp, never follow; rcu_sync / rcu_check_device then return
- * RCU_ERR_INVALID (error bit 0x8). */
+ * pool) they skip, read as zeros or clamp, never follow, and rows that have no place in the table are
+ * not stored; rcu_sync / rcu_check_device then return RCU_ERR_INVALID (error bit 0x8). */
 typedef struct rcu_seqs {
     const int32_t *cu;    /* [n_seq + 1]: rows cu[i] .. cu[i + 1] - 1 are sequence i's new tokens (none: equal) */
     const int32_t *len;   /* [n_seq]: positions of sequence i, its new tokens the last of them */

@@ -67,8 +67,11 @@ __global__ void __launch_bounds__(256) k_paged_store(const SeqView b, const T *_
     uint32_t first;
     const uint32_t n = seq_rows(b, seq, &first);
     if (t < first || t - first >= n) return;  // offsets out of order (reported)
-    const int32_t pos = seq_len(b, b.len[seq], n) - (int32_t)n + (int32_t)(t - first);
-    if (pos < 0) return;  // a length shorter than the new tokens (reported)
+    // a length that does not fit (reported): rows whose own position is outside the table are dropped
+    const int32_t len = b.len[seq];
+    seq_len(b, len, n);
+    const int64_t pos = (int64_t)len - n + (t - first);
+    if (pos < 0 || pos >= (int64_t)b.ld_pages << b.page_shift) return;
     const uint32_t pg = seq_page(b, seq, (uint32_t)(pos >> b.page_shift));
     if (pg == kNoRow) return;
     const uint32_t ps = 1u << b.page_shift, slot = (uint32_t)pos & (ps - 1);

@@ -590,3 +590,25 @@ def test_a_pool_of_another_device_is_refused(env):
                    lib.rcu_paged_store(other.ptr, pool, batch._ref, q.data_ptr(), q.data_ptr(), 0, 128)):
             assert st == 1 and b"another device" in lib.rcu_last_error(other.ptr)
     lib.rcu_paged_free(pool)
+
+
+@pytest.mark.parametrize("length", [50, 65, 1000, 2 ** 31 - 1, 2, -5, -2 ** 31])
+def test_a_wrong_length_overwrites_no_other_position(env, length):
+    """A table of three pages of 16, three new tokens and a length that does not fit: positions within the
+    table are written, the others dropped, and what lies in the pages stays."""
+    torch, rie, ctx = env
+    n_kv, hd, ps = 2, 64, 16
+    kp, vp = (torch.full((4, n_kv, ps, hd), x, dtype=torch.float16, device="cuda") for x in (1.0, 2.0))
+    cache = rie.PagedCache(ctx, n_kv, hd, ps, 4, k=kp, v=vp)
+    cu, ln, pages = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3], [length], [[2, 0, 3]]))
+    k = torch.arange(3, device="cuda").view(3, 1).expand(3, n_kv * hd).float() + 10
+    want_k, want_v = kp.clone(), vp.clone()
+    for t in range(3):
+        pos = length - 3 + t
+        if 0 <= pos < 48:
+            want_k[[2, 0, 3][pos // ps], :, pos % ps] = 10.0 + t
+            want_v[[2, 0, 3][pos // ps], :, pos % ps] = 20.0 + t
+    cache.store(rie.SeqBatch(cu, ln, pages, 3), k.contiguous(), (k + 10).contiguous())
+    with pytest.raises(rie.RcuError, match="0x8"):
+        ctx.sync()
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
