@@ -113,7 +113,7 @@ static int check_seqs(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *s, SeqV
     if (!pg || !s || !s->cu || !s->len || !s->pages) return set_err(ctx, RCU_ERR_INVALID, "null argument");
     if (ctx && pg->device != ctx->device) return set_err(ctx, RCU_ERR_INVALID, "paged cache: on another device than the context");
     if (int st = check_batch(ctx, s->n_tok, s->n_seq)) return st;
-    if (s->ld_pages == 0 || s->ld_pages * pg->page_size > 0x7fffffffull)
+    if (s->ld_pages == 0 || s->ld_pages > 0x7fffffffull / pg->page_size)
         return set_err(ctx, RCU_ERR_INVALID, "page table: 1 .. 2^31 / page_size pages a sequence");
     *v = SeqView{s->cu, s->len, s->pages, (uint32_t)s->n_seq, (uint32_t)s->n_tok, (uint32_t)s->ld_pages,
                  (uint32_t)pg->n_pages, pg->page_shift, ctx ? ctx->dev_err : nullptr};
