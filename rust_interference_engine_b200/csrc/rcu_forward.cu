@@ -1800,6 +1800,7 @@ int32_t rcu_backend_forward_device(rcu_backend *b, const uint32_t *tokens_dev, u
 
 int32_t rcu_backend_score(rcu_backend *b, const uint32_t *tokens, uint64_t n, uint64_t pos, const int32_t *targets,
                           float *logprob, float *entropy, uint64_t top_k, int32_t *top_ids, float *top_logprobs) {
+    RCU_GUARD_BEGIN
     if (!b || !tokens) return b ? set_err(b->ctx, RCU_ERR_INVALID, "null argument") : RCU_ERR_INVALID;
     if (!targets != !logprob) return set_err(b->ctx, RCU_ERR_INVALID, "score: pass targets and logprob, or neither");
     if (top_k && (!top_ids || !top_logprobs)) return set_err(b->ctx, RCU_ERR_INVALID, "score: top_k without its outputs");
@@ -1812,7 +1813,6 @@ int32_t rcu_backend_score(rcu_backend *b, const uint32_t *tokens, uint64_t n, ui
         if (targets && (targets[i] < -1 || targets[i] >= (int64_t)nv))
             return set_err(b->ctx, RCU_ERR_RUNTIME, "target id " + std::to_string(targets[i]) + " out of range");
     }
-    RCU_GUARD_BEGIN
     rcu_ctx *ctx = b->ctx;
     DeviceGuard guard(ctx);
     // results of one call, device and pinned host side by side: targets, logprob, entropy (max_batch
@@ -1856,7 +1856,7 @@ int32_t rcu_backend_score(rcu_backend *b, const uint32_t *tokens, uint64_t n, ui
         std::memcpy(top_logprobs, pin + 3 * T + T * top_k, T * top_k * 4);
     }
     return RCU_OK;
-    RCU_GUARD_END(b->ctx)
+    RCU_GUARD_END(b ? b->ctx : nullptr)
 }
 
 int32_t rcu_backend_forward_layers(rcu_backend *b, const float *x_dev, uint64_t n, uint64_t pos, uint64_t layer0,
