@@ -173,6 +173,22 @@ def test_target_outside_the_vocabulary_is_reported(env):
     ctx.sync()
 
 
+def test_logits_past_32_bits(env):
+    """Rows whose values lie more than 2^32 elements into the logits."""
+    torch = env[0]
+    rows, vocab = 29000, 151936
+    x = torch.zeros(rows, vocab, dtype=torch.float16, device="cuda")
+    pick = [0, 14000, 28400, rows - 1]
+    x[pick] = (torch.randn(len(pick), vocab, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda") * 4).half()
+    targets = np.random.default_rng(6).integers(0, vocab, rows)
+    got = run(env, x, targets, 3)
+    check(x[pick].float().cpu().numpy(), targets[pick], 3, {n: a[pick] for n, a in got.items()}, vocab)
+    rest = np.setdiff1d(np.arange(rows), pick)
+    step = (8 + vocab / 4096 + 64) * 2.0 ** -24  # equal values: -ln of the vocabulary, ties in order
+    assert (np.abs(got["logprob"][rest] + np.log(vocab)) <= step + 2.0 ** -23 * (1 + 2 * np.log(vocab))).all()
+    assert (got["top_ids"][rest] == np.arange(3)).all()
+
+
 @pytest.fixture(scope="module")
 def backend(env):
     torch, rie, ctx = env

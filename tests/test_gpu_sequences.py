@@ -612,3 +612,73 @@ def test_a_wrong_length_overwrites_no_other_position(env, length):
     with pytest.raises(rie.RcuError, match="0x8"):
         ctx.sync()
     assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+def test_the_largest_batch(env):
+    """16384 sequences, empty ones and a few chunks among them: append and attention."""
+    torch, rie, ctx = env
+    n_kv, n_head, hd, ps, n_seq = 1, 2, 64, 16, 1 << 14
+    rng = np.random.default_rng(40)
+    new = np.where(np.arange(n_seq) % 5 == 3, 0, 1)
+    new[[7, 9000, n_seq - 1]] = [20, 3, 5]
+    lens = new + rng.integers(0, 12, n_seq)
+    need = -(-lens // ps)
+    pages = np.zeros((n_seq, need.max()), dtype=np.int32)
+    order = rng.permutation(need.sum())
+    for i, at in enumerate(np.cumsum(need) - need):
+        pages[i, :need[i]] = order[at:at + need[i]]
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    n_tok = int(cu[-1])
+    pools = [torch.from_numpy(rng.standard_normal((int(need.sum()), n_kv, ps, hd)).astype(np.float16)).cuda() for _ in "kv"]
+    cache = rie.PagedCache(ctx, n_kv, hd, ps, int(need.sum()), k=pools[0], v=pools[1])
+    dev = [torch.from_numpy(x).cuda() for x in (cu, lens.astype(np.int32), pages)]
+    q, k, v = (torch.from_numpy(rng.standard_normal((n_tok, w)).astype(np.float32)).cuda() for w in (n_head * hd, hd, hd))
+    q /= 8
+    cache.store(rie.SeqBatch(*dev, n_tok), k, v)
+    out = torch.full_like(q, 7.5)
+    for max_new in (0, 1):
+        rie.paged_attention(ctx, cache, rie.SeqBatch(*dev, n_tok, max_new=max_new), q, n_head, out)
+        ctx.sync()
+        kn, vn = (x.double().cpu().numpy() for x in pools)
+        qn, got = q.double().cpu().numpy(), out.double().cpu().numpy()
+        for i in [*range(0, n_seq, 37), 7, 9000, n_seq - 1]:
+            rows = [(pages[i, p // ps], p % ps) for p in range(lens[i])]
+            ks, vs = (np.array([x[pg, :, sl] for pg, sl in rows]).reshape(-1, n_kv, hd) for x in (kn, vn))
+            assert (ks[lens[i] - new[i]:, 0] == k[cu[i]:cu[i + 1]].half().double().cpu().numpy()).all()
+            check_rows(got, qn, [ks], [vs], [(int(cu[i]), int(new[i]), int(lens[i]))], n_head, n_kv, hd, 0, 0.0, "f32")
+
+
+@pytest.mark.parametrize("ty", ["f32", "f16"])
+@pytest.mark.parametrize("n_head,n_kv,hd", [(300, 1, 32), (514, 2, 64), (129, 1, 256)])
+def test_groups_larger_than_a_tile(env, ty, n_head, n_kv, hd):
+    """One token's heads alone fill a tile of query rows, or more than one."""
+    c = Case(*env, [(1, 40), (3, 200), (1, 1)], n_head, n_kv, hd, 16, ty, seed=41)
+    c.check(c.run())
+    c.check(c.run(window=30), window=30)
+
+
+@pytest.mark.parametrize("new,ty", [(1, "f32"), (3, "f16"), (70, "f32"), (70, "f16")])
+def test_pools_past_32_bits(env, new, ty):
+    """Pages whose values lie more than 2^32 elements into the pool."""
+    torch, rie, ctx = env
+    n_kv, hd, ps, length = 1, 256, 1024, 1500
+    n_pages = (1 << 32) // (hd * ps) + 3
+    kp, vp = (torch.zeros(n_pages, n_kv, ps, hd, dtype=torch.float16, device="cuda") for _ in "kv")
+    g = torch.Generator(device="cuda").manual_seed(42)
+    k, v = (torch.randn(length, hd, generator=g, device="cuda").half() for _ in "kv")
+    cache = rie.PagedCache(ctx, n_kv, hd, ps, n_pages, k=kp, v=vp)
+    pages = torch.tensor([[n_pages - 1, n_pages - 2]], dtype=torch.int32, device="cuda")
+    for cu, ln in (([0, 1000], 1000), ([0, 500], 1500)):
+        cu, ln = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (cu, [ln]))
+        n, first = int(cu[1]), int(ln[0]) - int(cu[1])
+        cache.store(rie.SeqBatch(cu, ln, pages, n), k[first:first + n], v[first:first + n])
+    ctx.sync()
+    assert torch.equal(kp[n_pages - 1, 0], k[:ps]) and torch.equal(vp[n_pages - 2, 0, :length - ps], v[ps:])
+    assert not kp[:n_pages - 2].any()
+    q = (torch.randn(new, 2 * hd, generator=g, device="cuda") / 8).to(dtype(torch, ty))
+    out = torch.zeros_like(q)
+    cu, ln = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, new], [length]))
+    rie.paged_attention(ctx, cache, rie.SeqBatch(cu, ln, pages, new), q, 2, out)
+    ctx.sync()
+    check_rows(out.double().cpu().numpy(), q.double().cpu().numpy(), [k.view(-1, 1, hd).double().cpu().numpy()],
+               [v.view(-1, 1, hd).double().cpu().numpy()], [(0, new, length)], 2, 1, hd, 0, 0.0, ty)
