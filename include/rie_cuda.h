@@ -212,8 +212,8 @@ typedef struct rcu_seqs {
     const int32_t *len;   /* [n_seq]: positions of sequence i, its new tokens the last of them */
     const int32_t *pages; /* [n_seq][ld_pages]: position P of sequence i is in page pages[i][P / page_size] */
     uint64_t n_seq, n_tok, ld_pages;
-    uint64_t max_len;     /* the longest len, 0 when unknown: shapes the launch, never the results */
-    uint64_t max_new;     /* the most new tokens of a sequence, 0 when unknown: the same */
+    uint64_t max_len;     /* the longest len, 0 when unknown. Shapes the launch, and with it the order of sums: */
+    uint64_t max_new;     /* results differ by roundings alone. The most new tokens of a sequence, 0 when unknown: the same */
 } rcu_seqs;
 /* Appends the new tokens' keys and values (post-RoPE keys; rows of n_head_kv * head_dim values of
  * ggml type F32, F16 or BF16, ld values apart, every row on a 16-byte boundary), rounded once to
@@ -225,7 +225,11 @@ RCU_API int32_t rcu_paged_store(rcu_ctx *ctx, rcu_paged *pg, const rcu_seqs *seq
  * call, at most 16384 sequences. q_dev: n_tok rows of n_head * head_dim values (F32 or F16, already scaled by attn_scale),
  * ld_q apart; out_dev the same type, ld_out apart, and no part of q. window and softcap as in rcu_attention. Out rows
  * behind the last sequence stay as they were. Masked keys and values do not count, whatever they
- * hold. No workspace: calls may overlap on any streams. */
+ * hold; attended ones that are infinite or NaN give what the formula makes of them, at a cost: rows
+ * that such a value leaves not finite are computed again key by key (a NaN key costs nothing with f16
+ * queries). Sums are f32; the probabilities that weigh the values are rounded to f16 for f16 queries
+ * (relative 2^-11, as much as the output's own rounding) and carry 22 bits for f32 ones. No workspace:
+ * calls may overlap on any streams. */
 RCU_API int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu_seqs *seqs, const void *q_dev,
                                     uint32_t type, uint64_t ld_q, uint64_t n_head, uint64_t window, float softcap,
                                     void *out_dev, uint64_t ld_out);
@@ -233,7 +237,8 @@ RCU_API int32_t rcu_paged_attention(rcu_ctx *ctx, const rcu_paged *pg, const rcu
  * rows cu[i] .. cu[i + 1] - 1 (device, n_seq + 1 offsets) attend among themselves. q (F32 or F16
  * over F16 keys and values, or BF16 over BF16; already scaled), k, v and out are rows ld_q / ld_kv /
  * ld_out values apart, so slices of a fused projection do; out must not overlap them. max_len: the longest prompt, 0 when
- * unknown (shapes the launch only). */
+ * unknown (shapes the launch, as above). Roundings and values that are not finite as in
+ * rcu_paged_attention; bf16 queries round probabilities to bf16 (2^-8). */
 RCU_API int32_t rcu_packed_attention(rcu_ctx *ctx, const void *q_dev, uint32_t q_type, uint64_t ld_q,
                                      const void *k_dev, const void *v_dev, uint32_t kv_elem, uint64_t ld_kv,
                                      const int32_t *cu, uint64_t n_seq, uint64_t n_tok, uint64_t max_len,

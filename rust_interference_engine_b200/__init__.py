@@ -447,7 +447,8 @@ class SeqBatch:
     cu (n_seq + 1), len (n_seq) and pages (n_seq x width) are int32 CUDA tensors; the kernels read
     them when they run, so a captured graph replays with what they hold then. max_len (the longest
     len) and max_new (the most new tokens of one sequence), when the program knows them, shape the
-    launches, never the results."""
+    launches; results differ by roundings alone. Give max_new where sequences have a few new tokens
+    each: without it one of them is taken to have them all."""
 
     def __init__(self, cu, len, pages, n_tok: int, max_len: int = 0, max_new: int = 0):  # noqa: A002
         for x, what, dims in ((cu, "cu", 1), (len, "len", 1), (pages, "pages", 2)):

@@ -16,7 +16,9 @@
 //                16-bit values over S, each half handed on by itself.
 // While one tile's warps are at their softmax, the tensor core works on the other tile (CTA).
 // 16-bit queries: O stays in tensor memory; it is rescaled only when a row's maximum has grown by
-// more than 2^kTlLazy since its last rescale (p then is at most 2^(kTlLazy + kTlShift)).
+// more than 2^kTlLazy since its last rescale (p then is at most 2^(kTlLazy + kTlShift)). p is rounded
+// to the type of V, its sum is not: kind::f16 takes both operands in one type, and a second part of p
+// would double the products (as f32 queries do); 2^-11 or 2^-8 of p, as much as the output's rounding.
 // f32 queries: q (scaled by a power of two per row) and p are each split into two f16 parts, so each
 // product is two MMAs (head_dim above 128: Q's low part in the tensor memory that S and O leave); O is added up in registers block by block, because a long chain of additions
 // inside the tensor core, which does not round to nearest, would drift (8e-6 at 12k keys).
@@ -24,9 +26,10 @@
 // shared memory. All waits are bounded; TMEM is freed on every path.
 // Bound: a block's 4 x 128 x 128 x 128 products take 2048 cycles of the tensor pipe, and about 3000
 // pass, since a tile's S, softmax and P V follow one another and only the other tile's fill the gap;
-// one bf16 prompt of 8192 tokens, 32 heads of 128: 460 to 477 us (1.15 P/s). Run for seconds the
-// kernel meets the 1000 W limit (power cap active, 1.70 GHz) at 553 us; with constants in place of
-// the exponentials, or with fewer instructions in the issuing warp, the time was the same.
+// one bf16 prompt of 8192 tokens, 32 heads of 128: 547 to 551 us run for seconds, at the 1000 W limit
+// (power cap active, 1.70 GHz), and 460 to 487 us (1.15 P/s) in the first milliseconds; with constants in
+// place of the exponentials, or with fewer instructions in the issuing warp, the time was the same.
+// A softcap costs more than all of it (1800 us): tanhf for each score, for f32 queries twice.
 #include <cuda.h>
 
 #include <algorithm>
