@@ -299,7 +299,7 @@ __device__ __noinline__ void seq_attn_row(const SeqAttnParams &p, const SeqSpan 
         const E *src = reinterpret_cast<const E *>(x) + (uint64_t)(r == kNoRow ? 0 : r) * p.ld_kv + kvo;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            u[c] = __ldg(reinterpret_cast<const uint4 *>(src + 8 * min(sub + 8 * c, pieces - 1)));
+            u[c] = *reinterpret_cast<const uint4 *>(src + 8 * min(sub + 8 * c, pieces - 1));
             if (r == kNoRow || sub + 8 * c >= pieces) u[c] = make_uint4(0, 0, 0, 0);
         }
     };
