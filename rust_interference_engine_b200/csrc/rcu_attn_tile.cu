@@ -26,7 +26,7 @@
 // shared memory. All waits are bounded; TMEM is freed on every path.
 // Bound: a block's 4 x 128 x 128 x 128 products take 2048 cycles of the tensor pipe, and about 3000
 // pass, since a tile's S, softmax and P V follow one another and only the other tile's fill the gap;
-// one bf16 prompt of 8192 tokens, 32 heads of 128: 547 to 551 us run for seconds, at the 1000 W limit
+// one bf16 prompt of 8192 tokens, 32 heads of 128: 547 to 557 us run for seconds, at the 1000 W limit
 // (power cap active, 1.70 GHz), and 460 to 487 us (1.15 P/s) in the first milliseconds; with constants in
 // place of the exponentials, or with fewer instructions in the issuing warp, the time was the same.
 // A softcap costs more than all of it (1800 us): tanhf for each score, for f32 queries twice.
